@@ -35,6 +35,10 @@ extern "C" {
 #define MPR_ENOMEM (-3)   /* device allocation failed */
 #define MPR_EUNSUP (-4)   /* unsupported configuration */
 
+#define MPR_F32 0         /* dtype codes of the tensor operators */
+#define MPR_BF16 1
+#define MPR_F16 2
+
 typedef struct mpr_index mpr_index;
 typedef struct mpr_model mpr_model;
 
@@ -412,6 +416,62 @@ int mpr_gather_rows(const float* table, const int32_t* ids, int64_t n, int32_t d
                     void* stream);
 int mpr_embed_bwd(const float* dY, int32_t d, const int32_t* uniq, const int32_t* offs,
                   const int32_t* pos, int32_t n_uniq, float* dW, void* stream);
+
+/* ---- tensor operators for tuning and serving the reader (multimodalpromptretrieval_amd/ops.py;
+ * no reference counterpart: the reference trains with torch's own) ------------------------------
+ * dtype codes: 0 float32, 1 bfloat16, 2 float16; sums and statistics are 32 bits or wider.  All
+ * workspaces are the caller's, sized by the *_workspace calls, and hold nothing between calls, so
+ * calls on different streams and captured graphs share nothing.
+ *   mpr_embed_lookup: out[i, :] = scale * table[ids[i], :] (out [n, d], table row stride ld; ids
+ *   int32, or int64 with ids64).  An id outside [0, V) gives a row of NaN.
+ *   mpr_embed_grad: dtable[v, :] = scale * sum over ids[i] == v of dout[i, :] for all V rows (dout
+ *   row stride ld; rows without an id, padding_idx's (-1: none) among them, become 0), summed in
+ *   the order of the positions.
+ *   mpr_xattn_fwd / _bwd: attention of q [B, Lq, H, D] over k, v [B, Lk, Hkv, D], H a multiple of
+ *   Hkv, D a multiple of 8 up to 128, elements of a head contiguous; keep [B, Lk] bytes (0: the key
+ *   counts for nothing, whatever it holds) or NULL.  dims = {B, H, Hkv, Lq, Lk, D}; strides (in
+ *   elements) = {q batch, position, head, k .., v .., keep batch, dout batch, position, head (bwd
+ *   only)}.  out [B, Lq, H, D], lse [B, H, Lq] (base-2 log of the rows' sums; may be NULL in a
+ *   forward alone), dq as out (NULL: not wanted), dk / dv [B, Lk, Hkv, D] (both or none), all
+ *   contiguous.  A row without a key: 0.
+ *   mpr_logps_fwd: logps[s] = sum over t with labels[s, t] >= 0 of log softmax(logits[s, t])[label]
+ *   (logits [S, T, V] with strides xs, xt, 1; labels row stride ls; a label >= V gives NaN), and
+ *   row_stat [S, T, 2] for the backward.  With loss: sequences p and S / 2 + p are the chosen and
+ *   the rejected answer of pair p, margin = beta ((logps[p] - logps[S/2 + p]) - (ref[p] -
+ *   ref[S/2 + p])), loss = mean of -(1 - label_smoothing) log sigmoid(margin) - label_smoothing
+ *   log sigmoid(-margin), and dlogps [S] its derivative by logps.
+ *   mpr_logps_bwd: dlogits [S, T, V] = mult[0] (NULL: 1) * dlogps[s] * (onehot - softmax), 0 where
+ *   the label is ignored.
+ *   mpr_clip_grads: desc = n x {pointer, values, dtype, output pointer, output dtype} (int64): norm
+ *   = the L2 norm of all, output = value * min(1, max_norm / (norm + eps)).  The output may be the
+ *   tensor itself; no output anywhere (0): the norm alone.  Memory that overlaps is refused. */
+int mpr_embed_lookup(const void* table, int32_t dtype, int64_t V, int64_t ld, const void* ids,
+                     int32_t ids64, int64_t n, int32_t d, float scale, void* out, void* stream);
+int mpr_embed_grad_workspace(int32_t dtype, int64_t n, int64_t V, int32_t d, int64_t* bytes);
+int mpr_embed_grad(const void* dout, int32_t dtype, int64_t ld, const void* ids, int32_t ids64,
+                   int64_t n, int64_t V, int32_t d, float scale, int64_t padding_idx, void* dtable,
+                   void* ws, int64_t ws_bytes, void* stream);
+int mpr_xattn_workspace(const int64_t* dims, int32_t dtype, int64_t* fwd_bytes,
+                        int64_t* bwd_bytes);
+int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
+                  const int64_t* dims, const int64_t* strides, float scale, void* out, float* lse,
+                  void* ws, int64_t ws_bytes, void* stream);
+int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
+                  const int64_t* dims, const int64_t* strides, float scale, const void* out,
+                  const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                  int64_t ws_bytes, void* stream);
+int mpr_logps_workspace(int64_t S, int64_t T, int64_t V, int64_t* bytes);
+int mpr_logps_fwd(const void* logits, int32_t dtype, int64_t S, int64_t T, int64_t V, int64_t xs,
+                  int64_t xt, const void* labels, int32_t labels64, int64_t ls, float* logps,
+                  float* row_stat, const float* ref, double beta, double label_smoothing,
+                  float* loss, float* dlogps, void* ws, int64_t ws_bytes, void* stream);
+int mpr_logps_bwd(const void* logits, int32_t dtype, int64_t S, int64_t T, int64_t V, int64_t xs,
+                  int64_t xt, const void* labels, int32_t labels64, int64_t ls,
+                  const float* row_stat, const float* dlogps, const float* mult, void* dlogits,
+                  void* stream);
+int mpr_clip_workspace(int32_t n, const int64_t* desc, int64_t* bytes);
+int mpr_clip_grads(int32_t n, const int64_t* desc, double max_norm, double eps, float* norm,
+                   void* ws, int64_t ws_bytes, void* stream);
 
 /* ---- cosine_similarity with broadcasting (utils.py:57-62, every layout the reference takes;
  * the aligned-rows and [B,1,D] x [1,N,D] forms run mpr_cosine_rows / the index scan) ----

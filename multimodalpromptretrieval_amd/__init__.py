@@ -6,4 +6,4 @@ Python host surfaces mirror the reference (``T5VisionModel``, ``VQARetrieval`` w
 arithmetic runs in ``libmpr.so`` (hand-written gfx950 HIP kernels, C ABI in include/mpr.h).
 """
 # (``synthetic`` — seeded weights and inputs for tests and the bench — is not part of the API)
-__all__ = ["dataset", "encoders", "index", "model", "t5", "tokenization", "utils"]
+__all__ = ["dataset", "encoders", "index", "model", "ops", "t5", "tokenization", "utils"]

@@ -158,6 +158,29 @@ SIGNATURES = [
     ("mpr_gather_rows", c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p]),
     ("mpr_embed_bwd", c_int32, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_int32,
                                 c_void_p, c_void_p]),
+    ("mpr_embed_lookup", c_int32, [c_void_p, c_int32, c_int64, c_int64, c_void_p, c_int32,
+                                   c_int64, c_int32, c_float, c_void_p, c_void_p]),
+    ("mpr_embed_grad_workspace", c_int32, [c_int32, c_int64, c_int64, c_int32, I64P]),
+    ("mpr_embed_grad", c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int32, c_int64, c_int64,
+                                 c_int32, c_float, c_int64, c_void_p, c_void_p, c_int64,
+                                 c_void_p]),
+    ("mpr_xattn_workspace", c_int32, [I64P, c_int32, I64P, I64P]),
+    ("mpr_xattn_fwd", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, I64P, I64P,
+                                c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    ("mpr_xattn_bwd", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, I64P, I64P,
+                                c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p, c_int64, c_void_p]),
+    ("mpr_logps_workspace", c_int32, [c_int64, c_int64, c_int64, I64P]),
+    ("mpr_logps_fwd", c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
+                                ctypes.c_double, ctypes.c_double, c_void_p, c_void_p, c_void_p,
+                                c_int64, c_void_p]),
+    ("mpr_logps_bwd", c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p]),
+    ("mpr_clip_workspace", c_int32, [c_int32, I64P, I64P]),
+    ("mpr_clip_grads", c_int32, [c_int32, I64P, ctypes.c_double, ctypes.c_double, c_void_p,
+                                 c_void_p, c_int64, c_void_p]),
     ("mpr_dot_reduce", c_int32, [c_void_p, c_void_p, c_int32, I64P, I64P, I64P, c_int64,
                                  c_int64, c_int64, c_int32, c_void_p, c_void_p]),
     ("mpr_cos_combine", c_int32, [c_void_p, c_void_p, c_void_p, c_int32, I64P, I64P, I64P, I64P,

@@ -1,0 +1,949 @@
+// xattn.hip — attention of queries to another sequence's states (an encoder's), forward and
+// backward, for key / value heads that groups of query heads share.  Per (batch, key head), the
+// queries of its group are the rows r = g Lq + i (g < G = H / Hkv, i < Lq):
+//   S = scale q k^T,  P = softmax over the keys that the mask keeps,  O = P v;  no key kept: O = 0
+//   dV = P^T dO,  dS = P (dO v^T - rowsum(dO O)),  dQ = scale dS k,  dK = scale dS^T q
+// The softmax runs in one pass over the keys with a running maximum and sum (fp32, base 2), and
+// the backward computes P again from the saved row statistic lse2 = max + log2(sum), so nothing of
+// size Lq x Lk is kept.  A row of all shared heads of a group lies in one tile, so K and V are read
+// once for the group and dK, dV sum the heads in registers: no atomics, the same bits every run.
+//
+// Matrix products: bf16 inputs on v_mfma_f32_32x32x16_bf16, float and half inputs on
+// v_mfma_f32_32x32x2_f32 (exact fp32 products; half gradients would leave half's range as matrix
+// operands).  The products are arranged so that a tile's scores come out of the matrix core in the
+// lane order in which the next product takes them (scores transposed: lane = row, registers =
+// keys): probabilities go from one product to the next in registers, never through LDS.  P and dS
+// are rounded to bf16 as operands of the second products (half a step, 2^-9 relative each), as the
+// inputs are; sums stay fp32.
+//
+// Masked keys count for nothing whatever they hold (NaN, infinities): they are staged as zeros.
+#include <algorithm>
+#include <cmath>
+#include <type_traits>
+
+#include "ops.h"
+
+namespace mpr {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct XArgs {
+  const void *q, *k, *v, *dout, *o;
+  const uint8_t* keep;
+  int64_t q_bs, q_ls, q_hs, k_bs, k_ls, k_hs, v_bs, v_ls, v_hs, keep_bs, do_bs, do_ls, do_hs;
+  int B, H, Hkv, G, Lq, Lk, D;
+  int R;             // rows of a key head: G Lq
+  int tiles, splits, per_split;  // blocks along the tiled axis, and shares of the other one
+  float c;           // scale log2(e)
+  float scale;
+  void* out;         // forward: [B, Lq, H, D]
+  float* lse;        // [B, H, Lq]: max + log2(sum) of the scaled scores in base 2
+  float* delta;      // [B, H, Lq]
+  float *part, *part2;  // splits' shares
+  float* part_ms;    // [split][B Hkv R][2]: running maximum and sum
+  void *dq, *dk, *dv;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// ---- the two matrix cores ------------------------------------------------------------------------
+// A chunk is the contraction of one call; frag: a lane's share of it.  Lane l holds index l & 31 of
+// the operand's own axis; its half h = l >> 5 of the contraction.
+//   row(p, ld, ...): operand rows lie as rows of LDS, the contraction along them
+//   col(p, ld, ...): the contraction runs over rows of LDS, in the order in which a product's result
+//                    holds its rows: result register r of half h is row 8 (r / 4) + 4 h + r % 4
+struct MmaBf16 {
+  typedef bf16 elem;
+  typedef bf16x8 frag;
+  static constexpr int CHUNK = 16;  // contraction of a chunk
+  static constexpr int PAD = 8;     // elements between LDS rows: row and column reads spread banks
+  static __device__ __forceinline__ frag row(const elem* p, int ld, int r0, int c0, int lane) {
+    return *reinterpret_cast<const frag*>(p + (r0 + (lane & 31)) * ld + c0 + 8 * (lane >> 5));
+  }
+  // ds_read_tr16_b64: 16 lanes read 4 rows of 16 elements and each gets a column of them
+  static __device__ __forceinline__ frag col(const elem* p, int ld, int k0, int m0, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    const elem* a = p + (k0 + 4 * (g >> 1) + (i >> 2)) * ld + m0 + 16 * (g & 1) + 4 * (i & 3);
+    typedef __attribute__((address_space(3))) s16x4* lds4;
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)a);
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(a + 8 * ld));
+    const s16x8 z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_bit_cast(frag, z);
+  }
+  static __device__ __forceinline__ frag pack(const f32x16& x, int c) {
+    frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (bf16)x[8 * c + j];
+    return f;
+  }
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+struct MmaF32 {
+  typedef float elem;
+  typedef f32x4 frag;
+  static constexpr int CHUNK = 8;
+  static constexpr int PAD = 4;
+  static __device__ __forceinline__ frag row(const elem* p, int ld, int r0, int c0, int lane) {
+    return *reinterpret_cast<const frag*>(p + (r0 + (lane & 31)) * ld + c0 + 4 * (lane >> 5));
+  }
+  static __device__ __forceinline__ frag col(const elem* p, int ld, int k0, int m0, int lane) {
+    const elem* a = p + (k0 + 4 * (lane >> 5)) * ld + m0 + (lane & 31);
+    return frag{a[0], a[ld], a[2 * ld], a[3 * ld]};
+  }
+  static __device__ __forceinline__ frag pack(const f32x16& x, int c) {
+    return frag{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+  }
+  static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+// the row (0 .. 31) that result register r of this lane's half holds
+__device__ __forceinline__ int acc_row(int r, int lane) {
+  return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+}
+
+// ---- staging -------------------------------------------------------------------------------------
+// rows [r0, r0 + n) of a matrix of `rows` rows into LDS as M's elements; rows outside, rows that
+// `keep` drops and columns past D become zeros.  at(r): the row's first element.
+template <class T, class M, int DP, class At>
+__device__ __forceinline__ void stage(typename M::elem* lds, int n, int64_t r0, int64_t rows,
+                                      int D, const uint8_t* keep, At at, int t, int threads) {
+  typedef typename M::elem E;
+  constexpr int N = 8, CH = DP / N, LD = DP + M::PAD;
+  for (int i = t; i < n * CH; i += threads) {
+    const int r = i / CH, c = (i % CH) * N;
+    E x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = (E)0.f;
+    if (r0 + r < rows && c < D && (!keep || keep[r0 + r])) {
+      const typename Vec<T, N>::type v =
+          *reinterpret_cast<const typename Vec<T, N>::type*>(at(r0 + r) + c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) x[e] = (E)v[e];
+    }
+    E* o = lds + r * LD + c;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o[e] = x[e];
+  }
+}
+
+// a wave's 32 rows as second operands in registers: frag c = contraction chunk c of row lane & 31
+template <class T, class M, int DP>
+__device__ __forceinline__ void load_rows(typename M::frag (&f)[DP / M::CHUNK], const T* row,
+                                          bool in, int D, int lane) {
+  constexpr int N = M::CHUNK / 2;
+#pragma unroll
+  for (int c = 0; c < DP / M::CHUNK; ++c) {
+    const int d = c * M::CHUNK + N * (lane >> 5);
+#pragma unroll
+    for (int e = 0; e < N; ++e) f[c][e] = (typename M::elem)0.f;
+    if (in && d < D) {
+      const typename Vec<T, N>::type v =
+          *reinterpret_cast<const typename Vec<T, N>::type*>(row + d);
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[c][e] = (typename M::elem)v[e];
+    }
+  }
+}
+
+// bit i: key k0 + i exists and is kept (32 keys)
+__device__ __forceinline__ uint32_t keep_bits(const uint8_t* keep, int64_t k0, int Lk, int lane) {
+  const int64_t k = k0 + (lane & 31);
+  return (uint32_t)__ballot(k < Lk && (!keep || keep[k]));
+}
+
+// [tile | DP x 32 result, transposed] -> rows of 4-element runs: f(d, 4 values)
+template <int DP, class F>
+__device__ __forceinline__ void for_runs(const f32x16 (&acc)[DP / 32], int lane, F f) {
+#pragma unroll
+  for (int t = 0; t < DP / 32; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float x[4] = {acc[t][4 * r], acc[t][4 * r + 1], acc[t][4 * r + 2], acc[t][4 * r + 3]};
+      f(32 * t + 8 * r + 4 * (lane >> 5), x);
+    }
+}
+
+struct RowAt {  // row r of (b, key head): its query head and position
+  int h, i;
+};
+__device__ __forceinline__ RowAt row_at(const XArgs& a, int hk, int r) {
+  const int g = r / a.Lq;
+  return {hk * a.G + g, r - g * a.Lq};
+}
+
+// ---- forward -------------------------------------------------------------------------------------
+// A wave per 32 rows, the block's waves share the staged keys.
+template <class T, class M, int DP, int NW, int KT>
+__global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XArgs a) {
+  typedef typename M::elem E;
+  constexpr int LD = DP + M::PAD, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  __shared__ __align__(16) E ks[KT * LD];
+  __shared__ __align__(16) E vs[KT * LD];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int tile = blockIdx.x % a.tiles;
+  const int64_t rest = blockIdx.x / a.tiles;
+  const int split = (int)(rest % a.splits);
+  const int64_t bh = rest / a.splits;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
+  const int row = (tile * NW + wave) * 32 + (lane & 31);
+  const bool in = row < a.R;
+  const RowAt ra = row_at(a, hk, in ? row : 0);
+  const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
+  const uint8_t* keep = a.keep ? a.keep + b * a.keep_bs : nullptr;
+  typename M::frag q[NC];
+  load_rows<T, M, DP>(q, static_cast<const T*>(a.q) + b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs,
+                      in, a.D, lane);
+  f32x16 acc[DP / 32] = {};
+  float m = -INFINITY, l = 0.f;
+  const int k_lo = split * a.per_split, k_hi = min(a.Lk, k_lo + a.per_split);
+  for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
+    uint32_t bits[KT / 32];
+    uint32_t any = 0;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) any |= bits[u] = keep_bits(keep, k0 + 32 * u, k_hi, lane);
+    if (any == 0) continue;  // the same for every wave of the block
+    __syncthreads();
+    stage<T, M, DP>(ks, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return k + r * a.k_ls; }, t,
+                    64 * NW);
+    stage<T, M, DP>(vs, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return v + r * a.v_ls; }, t,
+                    64 * NW);
+    __syncthreads();
+    f32x16 s[KT / 32];
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) {
+      s[u] = f32x16{};
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+        s[u] = M::mma(M::row(ks, LD, 32 * u, c * M::CHUNK, lane), q[c], s[u]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = (bits[u] >> acc_row(r, lane)) & 1 ? s[u][r] * a.c : -INFINITY;
+        top = fmaxf(top, s[u][r]);
+      }
+    }
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float base = top == -INFINITY ? 0.f : top;
+    const float alpha = exp2_fast(m - base);
+    m = top;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = exp2_fast(s[u][r] - base);
+        sum += s[u][r];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) acc[d] *= alpha;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u)
+#pragma unroll
+      for (int c = 0; c < PC; ++c) {
+        const typename M::frag p = M::pack(s[u], c);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+          acc[d] = M::mma(M::col(vs, LD, 32 * u + c * M::CHUNK, 32 * d, lane), p, acc[d]);
+      }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!in) return;
+  if (a.splits > 1) {
+    const int64_t at = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
+    float* o = a.part + at * a.D;
+    for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
+      if (d < a.D) store_f<float, 4>(o + d, x);
+    });
+    if (lane < 32) {
+      a.part_ms[2 * at] = m;
+      a.part_ms[2 * at + 1] = l;
+    }
+    return;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* o = static_cast<T*>(a.out) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+  for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
+    const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
+    if (d < a.D) store_f<T, 4>(o + d, y);
+  });
+  if (lane < 32 && a.lse)
+    a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+
+// The splits of a row: rescaled to their common maximum and summed in order.  A wave per row.
+template <class T>
+__global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.R;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  float m = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ms[2 * (s * rows + at)]);
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, o[2] = {0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t p = s * rows + at;
+    const float w = exp2_fast(a.part_ms[2 * p] - base);
+    l += w * a.part_ms[2 * p + 1];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int d = lane + 64 * j;
+      if (d < a.D) o[j] += w * a.part[p * a.D + d];
+    }
+  }
+  const int64_t bh = at / a.R;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
+  const RowAt ra = row_at(a, hk, (int)(at % a.R));
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(a.out) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int d = lane + 64 * j;
+    if (d < a.D) out[d] = from_f<T>(o[j] * inv);
+  }
+  if (lane == 0 && a.lse)
+    a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+
+// ---- a few rows (single tokens) ------------------------------------------------------------------
+// The keys and values are read once and that is all the time there is: no matrix core, no LDS until
+// the end.  LPR lanes read a key's row, 16 bytes each, so a wave reads 64 / LPR keys at a time; each
+// such group of lanes keeps its own running maximum, sum and output share of every row, and they
+// are joined when the keys are done.
+constexpr int FEW_WAVES = 4, FEW_AHEAD = 4;
+template <class T, int LPR, int NR>
+__global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
+  constexpr int N = VEC16<T>, KPI = 64 / LPR;
+  __shared__ float so[FEW_WAVES][NR][LPR * N];
+  __shared__ float sm[FEW_WAVES][NR][2];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int64_t rest = blockIdx.x;
+  const int split = (int)(rest % a.splits);
+  const int64_t bh = rest / a.splits;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
+  const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
+  const uint8_t* keep = a.keep ? a.keep + b * a.keep_bs : nullptr;
+  const int d0 = (lane % LPR) * N, sub = lane / LPR;
+  const bool act = d0 < a.D;
+  float q[NR][N], o[NR][N], m[NR], l[NR];
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) q[r][e] = o[r][e] = 0.f;
+    if (r < a.R && act) {
+      const RowAt ra = row_at(a, hk, r);
+      load_f<T, N>(static_cast<const T*>(a.q) + b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs + d0,
+                   q[r]);
+#pragma unroll
+      for (int e = 0; e < N; ++e) q[r][e] *= a.c;
+    }
+  }
+  const int k_lo = split * a.per_split, k_hi = min(a.Lk, k_lo + a.per_split);
+  for (int k0 = k_lo + wave * KPI * FEW_AHEAD; k0 < k_hi; k0 += FEW_WAVES * KPI * FEW_AHEAD) {
+    typename Vec<T, N>::type kx[FEW_AHEAD], vx[FEW_AHEAD];
+    bool ok[FEW_AHEAD];
+#pragma unroll
+    for (int u = 0; u < FEW_AHEAD; ++u) {
+      const int64_t key = k0 + u * KPI + sub;
+      ok[u] = key < k_hi && (!keep || keep[key]);
+      kx[u] = vx[u] = typename Vec<T, N>::type{};
+      if (ok[u] && act) {
+        kx[u] = *reinterpret_cast<const typename Vec<T, N>::type*>(k + key * a.k_ls + d0);
+        vx[u] = *reinterpret_cast<const typename Vec<T, N>::type*>(v + key * a.v_ls + d0);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+      float s[FEW_AHEAD], top = m[r];
+#pragma unroll
+      for (int u = 0; u < FEW_AHEAD; ++u) {
+        float x = 0.f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) x = fmaf(q[r][e], vec_f<T, N>(kx[u], e), x);
+#pragma unroll
+        for (int off = 1; off < LPR; off <<= 1) x += __shfl_xor(x, off, 64);
+        s[u] = ok[u] ? x : -INFINITY;
+        top = fmaxf(top, s[u]);
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      const float alpha = exp2_fast(m[r] - base);
+      m[r] = top;
+      l[r] *= alpha;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[r][e] *= alpha;
+#pragma unroll
+      for (int u = 0; u < FEW_AHEAD; ++u) {
+        const float p = exp2_fast(s[u] - base);
+        l[r] += p;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[r][e] = fmaf(p, vec_f<T, N>(vx[u], e), o[r][e]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < NR; ++r) {  // the wave's groups of lanes
+#pragma unroll
+    for (int off = LPR; off < 64; off <<= 1) {
+      const float m2 = __shfl_xor(m[r], off, 64), l2 = __shfl_xor(l[r], off, 64);
+      const float top = fmaxf(m[r], m2), base = top == -INFINITY ? 0.f : top;
+      const float w = exp2_fast(m[r] - base), w2 = exp2_fast(m2 - base);
+      m[r] = top;
+      l[r] = l[r] * w + l2 * w2;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o[r][e] = o[r][e] * w + __shfl_xor(o[r][e], off, 64) * w2;
+    }
+    if (lane < LPR)
+#pragma unroll
+      for (int e = 0; e < N; ++e) so[wave][r][d0 + e] = o[r][e];
+    if (lane == 0) {
+      sm[wave][r][0] = m[r];
+      sm[wave][r][1] = l[r];
+    }
+  }
+  __syncthreads();
+  for (int i = t; i < a.R * a.D; i += 64 * FEW_WAVES) {  // the block's waves
+    const int r = i / a.D, d = i - r * a.D;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w) top = fmaxf(top, sm[w][r][0]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float x = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; ++w) {
+      const float f = exp2_fast(sm[w][r][0] - base);
+      x += f * so[w][r][d];
+      sum += f * sm[w][r][1];
+    }
+    if (a.splits > 1) {
+      const int64_t at = ((int64_t)split * a.B * a.Hkv + bh) * a.R + r;
+      a.part[at * a.D + d] = x;
+      if (d == 0) {
+        a.part_ms[2 * at] = top;
+        a.part_ms[2 * at + 1] = sum;
+      }
+    } else {
+      const RowAt ra = row_at(a, hk, r);
+      static_cast<T*>(a.out)[(((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D + d] =
+          from_f<T>(sum == 0.f ? 0.f : x / sum);
+      if (d == 0 && a.lse)
+        a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] =
+            sum == 0.f ? -INFINITY : top + log2f(sum);
+    }
+  }
+}
+
+// ---- backward ------------------------------------------------------------------------------------
+// delta[b, h, i] = sum_d dO O.  16 lanes a row.
+template <class T>
+__global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
+  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, i, h)
+  const int c = threadIdx.x & 15;
+  float s = 0.f;
+  const bool in = row < (int64_t)a.B * a.Lq * a.H;
+  const int h = (int)(row % a.H);
+  const int64_t bi = row / a.H;
+  const int i = (int)(bi % a.Lq), b = (int)(bi / a.Lq);
+  if (in && 8 * c < a.D) {
+    float x[8], y[8];
+    load_f<T, 8>(static_cast<const T*>(a.o) + row * a.D + 8 * c, x);
+    load_f<T, 8>(static_cast<const T*>(a.dout) + b * a.do_bs + i * a.do_ls + h * a.do_hs + 8 * c,
+                 y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+  }
+#pragma unroll
+  for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off, 64);
+  if (in && c == 0) a.delta[((int64_t)b * a.H + h) * a.Lq + i] = s;
+}
+
+// dQ: a wave per 32 rows, over the keys.
+template <class T, class M, int DP, int NW, int KT>
+__global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XArgs a) {
+  typedef typename M::elem E;
+  constexpr int LD = DP + M::PAD, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  __shared__ __align__(16) E ks[KT * LD];
+  __shared__ __align__(16) E vs[KT * LD];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int tile = blockIdx.x % a.tiles;
+  const int64_t rest = blockIdx.x / a.tiles;
+  const int split = (int)(rest % a.splits);
+  const int64_t bh = rest / a.splits;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
+  const int row = (tile * NW + wave) * 32 + (lane & 31);
+  const bool in = row < a.R;
+  const RowAt ra = row_at(a, hk, in ? row : 0);
+  const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
+  const uint8_t* keep = a.keep ? a.keep + b * a.keep_bs : nullptr;
+  typename M::frag q[NC], go[NC];
+  load_rows<T, M, DP>(q, static_cast<const T*>(a.q) + b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs,
+                      in, a.D, lane);
+  load_rows<T, M, DP>(go,
+                      static_cast<const T*>(a.dout) + b * a.do_bs + ra.i * a.do_ls +
+                          ra.h * a.do_hs,
+                      in, a.D, lane);
+  const int64_t stat = ((int64_t)b * a.H + ra.h) * a.Lq + ra.i;
+  const float lse = in ? a.lse[stat] : -INFINITY, delta = in ? a.delta[stat] : 0.f;
+  const bool some = lse != -INFINITY;
+  f32x16 acc[DP / 32] = {};
+  const int k_lo = split * a.per_split, k_hi = min(a.Lk, k_lo + a.per_split);
+  for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
+    uint32_t bits[KT / 32];
+    uint32_t any = 0;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) any |= bits[u] = keep_bits(keep, k0 + 32 * u, k_hi, lane);
+    if (any == 0) continue;
+    __syncthreads();
+    stage<T, M, DP>(ks, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return k + r * a.k_ls; }, t,
+                    64 * NW);
+    stage<T, M, DP>(vs, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return v + r * a.v_ls; }, t,
+                    64 * NW);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        s = M::mma(M::row(ks, LD, 32 * u, c * M::CHUNK, lane), q[c], s);
+        dp = M::mma(M::row(vs, LD, 32 * u, c * M::CHUNK, lane), go[c], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const bool ok = ((bits[u] >> acc_row(r, lane)) & 1) && some;
+        s[r] = ok ? exp2_fast(fmaf(s[r], a.c, -lse)) * (dp[r] - delta) : 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < PC; ++c) {
+        const typename M::frag ds = M::pack(s, c);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d)
+          acc[d] = M::mma(M::col(ks, LD, 32 * u + c * M::CHUNK, 32 * d, lane), ds, acc[d]);
+      }
+    }
+  }
+  if (!in) return;
+  if (a.splits > 1) {
+    float* o = a.part + (((int64_t)split * a.B * a.Hkv + bh) * a.R + row) * a.D;
+    for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
+      if (d < a.D) store_f<float, 4>(o + d, x);
+    });
+    return;
+  }
+  T* o = static_cast<T*>(a.dq) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+  for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
+    const float y[4] = {x[0] * a.scale, x[1] * a.scale, x[2] * a.scale, x[3] * a.scale};
+    if (d < a.D) store_f<T, 4>(o + d, y);
+  });
+}
+
+// dK, dV: a wave per 32 keys, over the rows of every head that shares them.
+template <class T, class M, int DP, int NW, int RT>
+__global__ __launch_bounds__(64 * NW) void xattn_dkv_kernel(XArgs a) {
+  typedef typename M::elem E;
+  constexpr int LD = DP + M::PAD, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  __shared__ __align__(16) E qs[RT * LD];
+  __shared__ __align__(16) E gs[RT * LD];
+  __shared__ __align__(16) float st[2][RT];  // lse, delta
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int tile = blockIdx.x % a.tiles;
+  const int64_t rest = blockIdx.x / a.tiles;
+  const int split = (int)(rest % a.splits);
+  const int64_t bh = rest / a.splits;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
+  const int key = (tile * NW + wave) * 32 + (lane & 31);
+  const bool in = key < a.Lk;
+  const bool ok = in && (!a.keep || a.keep[b * a.keep_bs + key]);
+  typename M::frag k[NC], v[NC];
+  load_rows<T, M, DP>(k, static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs + key * a.k_ls, ok,
+                      a.D, lane);
+  load_rows<T, M, DP>(v, static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs + key * a.v_ls, ok,
+                      a.D, lane);
+  const T* q = static_cast<const T*>(a.q) + b * a.q_bs;
+  const T* go = static_cast<const T*>(a.dout) + b * a.do_bs;
+  f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
+  const int r_lo = split * a.per_split, r_hi = min(a.R, r_lo + a.per_split);
+  const bool live = __syncthreads_or(ok);  // a tile of padding has no gradient
+  for (int r0 = r_lo; live && r0 < r_hi; r0 += RT) {
+    __syncthreads();
+    stage<T, M, DP>(qs, RT, r0, r_hi, a.D, nullptr, [&](int64_t r) {
+      const RowAt ra = row_at(a, hk, (int)r);
+      return q + ra.i * a.q_ls + ra.h * a.q_hs;
+    }, t, 64 * NW);
+    stage<T, M, DP>(gs, RT, r0, r_hi, a.D, nullptr, [&](int64_t r) {
+      const RowAt ra = row_at(a, hk, (int)r);
+      return go + ra.i * a.do_ls + ra.h * a.do_hs;
+    }, t, 64 * NW);
+    for (int i = t; i < RT; i += 64 * NW) {
+      const bool there = r0 + i < r_hi;
+      const RowAt ra = row_at(a, hk, there ? r0 + i : 0);
+      const int64_t at = ((int64_t)b * a.H + ra.h) * a.Lq + ra.i;
+      st[0][i] = there ? a.lse[at] : -INFINITY;
+      st[1][i] = there ? a.delta[at] : 0.f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < RT / 32; ++u) {
+      f32x16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        s = M::mma(M::row(qs, LD, 32 * u, c * M::CHUNK, lane), k[c], s);
+        dp = M::mma(M::row(gs, LD, 32 * u, c * M::CHUNK, lane), v[c], dp);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = 32 * u + acc_row(r, lane);
+        const float lse = st[0][i];
+        const bool p = ok && lse != -INFINITY;
+        s[r] = p ? exp2_fast(fmaf(s[r], a.c, -lse)) : 0.f;
+        dp[r] = p ? s[r] * (dp[r] - st[1][i]) : 0.f;
+      }
+#pragma unroll
+      for (int c = 0; c < PC; ++c) {
+        const typename M::frag p = M::pack(s, c), ds = M::pack(dp, c);
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) {
+          dv[d] = M::mma(M::col(gs, LD, 32 * u + c * M::CHUNK, 32 * d, lane), p, dv[d]);
+          dk[d] = M::mma(M::col(qs, LD, 32 * u + c * M::CHUNK, 32 * d, lane), ds, dk[d]);
+        }
+      }
+    }
+  }
+  if (!in) return;
+  if (a.splits > 1) {
+    const int64_t at = (((int64_t)split * a.B * a.Hkv + bh) * a.Lk + key) * a.D;
+    for_runs<DP>(dk, lane, [&](int d, const float (&x)[4]) {
+      if (d < a.D) store_f<float, 4>(a.part + at + d, x);
+    });
+    for_runs<DP>(dv, lane, [&](int d, const float (&x)[4]) {
+      if (d < a.D) store_f<float, 4>(a.part2 + at + d, x);
+    });
+    return;
+  }
+  const int64_t at = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
+  for_runs<DP>(dk, lane, [&](int d, const float (&x)[4]) {
+    const float y[4] = {x[0] * a.scale, x[1] * a.scale, x[2] * a.scale, x[3] * a.scale};
+    if (d < a.D) store_f<T, 4>(static_cast<T*>(a.dk) + at + d, y);
+  });
+  for_runs<DP>(dv, lane, [&](int d, const float (&x)[4]) {
+    if (d < a.D) store_f<T, 4>(static_cast<T*>(a.dv) + at + d, x);
+  });
+}
+
+// The splits' shares of a gradient, summed in order.  rows: (b, key head, r); kind 0: dQ rows,
+// 1: dK and dV rows.
+template <class T>
+__global__ __launch_bounds__(256) void xattn_sum_kernel(XArgs a, int kind) {
+  const int n = kind == 0 ? a.R : a.Lk;
+  const int64_t rows = (int64_t)a.B * a.Hkv * n;
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= rows * a.D) return;
+  const int64_t at = i / a.D;
+  const int d = (int)(i - at * a.D);
+  const int64_t bh = at / n;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv), r = (int)(at % n);
+  float x[4] = {}, y[4] = {};
+  for (int s = 0; s < a.splits; ++s) {
+    float f[4];
+    load_f<float, 4>(a.part + s * rows * a.D + i, f);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] += f[e];
+    if (kind == 1) {
+      load_f<float, 4>(a.part2 + s * rows * a.D + i, f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += f[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] *= a.scale;
+  if (kind == 0) {
+    const RowAt ra = row_at(a, hk, r);
+    store_f<T, 4>(static_cast<T*>(a.dq) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D + d, x);
+  } else {
+    const int64_t o = (((int64_t)b * a.Lk + r) * a.Hkv + hk) * a.D + d;
+    store_f<T, 4>(static_cast<T*>(a.dk) + o, x);
+    store_f<T, 4>(static_cast<T*>(a.dv) + o, y);
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+constexpr int FEW_ROWS = 8;  // rows of a key head that the single-token kernel takes
+
+// Blocks along one axis and shares of the other: where the tiles alone leave the chip idle, the
+// other axis is split (at least `least` of it a share, a multiple of `unit`) and joined afterwards.
+struct Tiling {
+  int nw = 1, tiles = 1, splits = 1, per = 0;
+};
+Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t least, int unit) {
+  Tiling t;
+  t.nw = n <= 32 ? 1 : n <= 64 ? 2 : 4;
+  t.tiles = (int)std::max<int64_t>(1, cdiv(n, 32 * t.nw));
+  int64_t s = cdiv(want, std::max<int64_t>(1, heads * t.tiles));
+  s = std::max<int64_t>(1, std::min(s, other / least));
+  t.per = (int)(cdiv(cdiv(std::max<int64_t>(other, 1), s), unit) * unit);
+  t.splits = (int)std::max<int64_t>(1, cdiv(other, t.per));
+  return t;
+}
+
+struct XPlan {
+  Tiling fwd, dq, dkv;
+  bool few;
+  int64_t fwd_bytes, bwd_bytes, part2, part_ms, delta;  // offsets
+};
+
+int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+XPlan xattn_plan(const int64_t* dims) {
+  const int64_t B = dims[0], H = dims[1], Hkv = dims[2], Lq = dims[3], Lk = dims[4], D = dims[5];
+  const int64_t heads = B * Hkv, R = H / Hkv * Lq;
+  XPlan p;
+  p.few = R <= FEW_ROWS;
+  if (p.few) {
+    p.fwd = tiling(heads, 1, Lk, 1024, 256, 64);
+    p.fwd.tiles = 1;
+  } else {
+    p.fwd = tiling(heads, R, Lk, 512, 128, 64);
+  }
+  p.dq = tiling(heads, R, Lk, 512, 128, 64);
+  p.dkv = tiling(heads, Lk, R, 512, 128, 64);
+  int64_t at = 0;
+  if (p.fwd.splits > 1) at = up256(p.fwd.splits * heads * R * D * 4);
+  p.part_ms = at;
+  p.fwd_bytes = at + (p.fwd.splits > 1 ? p.fwd.splits * heads * R * 8 : 0);
+  p.delta = 0;
+  const int64_t base = up256(B * H * Lq * 4);
+  int64_t part = p.dq.splits > 1 ? p.dq.splits * heads * R * D * 4 : 0;
+  int64_t kv = p.dkv.splits > 1 ? up256(p.dkv.splits * heads * Lk * D * 4) : 0;
+  p.part2 = base + kv;
+  p.bwd_bytes = base + std::max(part, 2 * kv);
+  return p;
+}
+
+int xattn_check(const char* what, const int64_t* dims, int32_t dtype) {
+  MPR_REQUIRE(dims, "%s: no dimensions", what);
+  MPR_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype code %d", what, (int)dtype);
+  const int64_t B = dims[0], H = dims[1], Hkv = dims[2], Lq = dims[3], Lk = dims[4], D = dims[5];
+  const int64_t most = (int64_t)1 << 30;
+  MPR_REQUIRE(B >= 0 && B <= most && Lq >= 0 && Lq <= most && Lk >= 0 && Lk <= most,
+              "%s: B=%lld Lq=%lld Lk=%lld", what, (long long)B, (long long)Lq, (long long)Lk);
+  MPR_REQUIRE(Hkv >= 1 && H >= Hkv && H % Hkv == 0 && H <= 65536,
+              "%s: %lld query heads over %lld key heads", what, (long long)H, (long long)Hkv);
+  MPR_REQUIRE(D >= 8 && D <= 128 && D % 8 == 0, "%s: head dim %lld (a multiple of 8 up to 128)",
+              what, (long long)D);
+  MPR_REQUIRE(H / Hkv * Lq <= most && B * Hkv <= most, "%s: too many rows", what);
+  const XPlan p = xattn_plan(dims);
+  for (const Tiling& t : {p.fwd, p.dq, p.dkv})
+    MPR_REQUIRE(B * Hkv <= MAX_GRID_X / ((int64_t)t.tiles * t.splits), "%s: too many blocks", what);
+  return MPR_OK;
+}
+
+XArgs xattn_args(const void* q, const void* k, const void* v, const uint8_t* keep,
+                 const int64_t* dims, const int64_t* st, float scale) {
+  XArgs a{};
+  a.q = q; a.k = k; a.v = v; a.keep = keep;
+  a.q_bs = st[0]; a.q_ls = st[1]; a.q_hs = st[2];
+  a.k_bs = st[3]; a.k_ls = st[4]; a.k_hs = st[5];
+  a.v_bs = st[6]; a.v_ls = st[7]; a.v_hs = st[8];
+  a.keep_bs = st[9];
+  a.B = (int)dims[0]; a.H = (int)dims[1]; a.Hkv = (int)dims[2];
+  a.Lq = (int)dims[3]; a.Lk = (int)dims[4]; a.D = (int)dims[5];
+  a.G = a.H / a.Hkv;
+  a.R = a.G * a.Lq;
+  a.scale = scale;
+  a.c = scale * LOG2E;
+  return a;
+}
+
+unsigned xattn_tile(XArgs& a, const Tiling& t) {
+  a.tiles = t.tiles;
+  a.splits = t.splits;
+  a.per_split = t.per;
+  return (unsigned)((int64_t)a.B * a.Hkv * t.tiles * t.splits);
+}
+
+// Storage type -> matrix core.
+template <class T>
+struct MmaOf { typedef MmaF32 type; };
+template <>
+struct MmaOf<bf16> { typedef MmaBf16 type; };
+
+// f(integral constant DP, integral constant NW)
+template <class F>
+int by_tile(int D, int nw, F&& f) {
+  using std::integral_constant;
+  if (D <= 64) {
+    if (nw == 1) return f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (nw == 2) return f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    return f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  }
+  if (nw == 1) return f(integral_constant<int, 128>{}, integral_constant<int, 1>{});
+  if (nw == 2) return f(integral_constant<int, 128>{}, integral_constant<int, 2>{});
+  return f(integral_constant<int, 128>{}, integral_constant<int, 4>{});
+}
+
+template <class T, int NR>
+int few_rows(const XArgs& a, unsigned blocks, hipStream_t s) {
+  constexpr int N = VEC16<T>;
+  const dim3 grid(blocks), block(64 * FEW_WAVES);
+  if (a.D <= 8 * N) xattn_few_kernel<T, 8, NR><<<grid, block, 0, s>>>(a);
+  else if (a.D <= 16 * N) xattn_few_kernel<T, 16, NR><<<grid, block, 0, s>>>(a);
+  else xattn_few_kernel<T, 32, NR><<<grid, block, 0, s>>>(a);
+  MPR_LAUNCHED();
+  return MPR_OK;
+}
+
+template <class T>
+int xattn_forward(XArgs a, const XPlan& p, hipStream_t s) {
+  typedef typename MmaOf<T>::type M;
+  constexpr int KT = sizeof(typename M::elem) == 2 ? 64 : 32;
+  const unsigned blocks = xattn_tile(a, p.fwd);
+  if (p.few) {
+    MPR_TRY(a.R == 1 ? (few_rows<T, 1>(a, blocks, s)) : a.R == 2 ? (few_rows<T, 2>(a, blocks, s))
+            : a.R <= 4 ? (few_rows<T, 4>(a, blocks, s)) : (few_rows<T, 8>(a, blocks, s)));
+  } else {
+    MPR_TRY(by_tile(a.D, p.fwd.nw, [&](auto dp, auto nw) -> int {
+      constexpr int DP = dp, NW = nw;
+      xattn_fwd_kernel<T, M, DP, NW, NW == 4 ? KT : 32><<<blocks, 64 * NW, 0, s>>>(a);
+      MPR_LAUNCHED();
+      return MPR_OK;
+    }));
+  }
+  if (a.splits > 1) {
+    const int64_t rows = (int64_t)a.B * a.Hkv * a.R;
+    xattn_join_kernel<T><<<dim3((unsigned)cdiv(rows, 4)), 256, 0, s>>>(a);
+    MPR_LAUNCHED();
+  }
+  return MPR_OK;
+}
+
+template <class T>
+int xattn_backward(XArgs a, const XPlan& p, hipStream_t s) {
+  typedef typename MmaOf<T>::type M;
+  constexpr int KT = sizeof(typename M::elem) == 2 ? 64 : 32;
+  const int64_t rows = (int64_t)a.B * a.Lq * a.H, heads = (int64_t)a.B * a.Hkv;
+  if (rows) {
+    xattn_delta_kernel<T><<<dim3((unsigned)cdiv(rows, 16)), 256, 0, s>>>(a);
+    MPR_LAUNCHED();
+  }
+  if (a.Lk && a.dk) {
+    const unsigned blocks = xattn_tile(a, p.dkv);
+    MPR_TRY(by_tile(a.D, p.dkv.nw, [&](auto dp, auto nw) -> int {
+      constexpr int DP = dp, NW = nw;
+      xattn_dkv_kernel<T, M, DP, NW, 32><<<blocks, 64 * NW, 0, s>>>(a);
+      MPR_LAUNCHED();
+      return MPR_OK;
+    }));
+    if (a.splits > 1) {
+      xattn_sum_kernel<T><<<dim3((unsigned)cdiv(heads * a.Lk * a.D, 1024)), 256, 0, s>>>(a, 1);
+      MPR_LAUNCHED();
+    }
+  }
+  if (rows && a.dq) {
+    const unsigned blocks = xattn_tile(a, p.dq);
+    MPR_TRY(by_tile(a.D, p.dq.nw, [&](auto dp, auto nw) -> int {
+      constexpr int DP = dp, NW = nw;
+      xattn_dq_kernel<T, M, DP, NW, NW == 4 ? KT : 32><<<blocks, 64 * NW, 0, s>>>(a);
+      MPR_LAUNCHED();
+      return MPR_OK;
+    }));
+    if (a.splits > 1) {
+      xattn_sum_kernel<T><<<dim3((unsigned)cdiv(heads * a.R * a.D, 1024)), 256, 0, s>>>(a, 0);
+      MPR_LAUNCHED();
+    }
+  }
+  return MPR_OK;
+}
+
+}  // namespace
+}  // namespace mpr
+
+using namespace mpr;
+
+extern "C" {
+
+int mpr_xattn_workspace(const int64_t* dims, int32_t dtype, int64_t* fwd_bytes,
+                        int64_t* bwd_bytes) {
+  return ops_call("xattn_workspace", [&]() -> int {
+    MPR_TRY(xattn_check("xattn_workspace", dims, dtype));
+    MPR_REQUIRE(fwd_bytes && bwd_bytes, "xattn_workspace: null pointer");
+    const XPlan p = xattn_plan(dims);
+    *fwd_bytes = p.fwd_bytes;
+    *bwd_bytes = p.bwd_bytes;
+    return MPR_OK;
+  });
+}
+
+int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
+                  const int64_t* dims, const int64_t* strides, float scale, void* out, float* lse,
+                  void* ws, int64_t ws_bytes, void* stream) {
+  return ops_call("xattn_fwd", [&]() -> int {
+    MPR_TRY(xattn_check("xattn_fwd", dims, dtype));
+    MPR_REQUIRE(strides, "xattn_fwd: no strides");
+    if (dims[0] * dims[3] == 0) return MPR_OK;
+    MPR_REQUIRE(q && out && (dims[4] == 0 || (k && v)), "xattn_fwd: null pointer");
+    const XPlan p = xattn_plan(dims);
+    MPR_REQUIRE(p.fwd_bytes == 0 || (ws && ws_bytes >= p.fwd_bytes),
+                "xattn_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
+                (long long)p.fwd_bytes);
+    XArgs a = xattn_args(q, k, v, keep, dims, strides, scale);
+    a.out = out;
+    a.lse = lse;
+    a.part = static_cast<float*>(ws);
+    a.part_ms = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part_ms);
+    return by_dtype(dtype, [&](auto z) -> int {
+      return xattn_forward<decltype(z)>(a, p, op_stream(stream));
+    });
+  });
+}
+
+int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
+                  const int64_t* dims, const int64_t* strides, float scale, const void* out,
+                  const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                  int64_t ws_bytes, void* stream) {
+  return ops_call("xattn_bwd", [&]() -> int {
+    MPR_TRY(xattn_check("xattn_bwd", dims, dtype));
+    MPR_REQUIRE(strides, "xattn_bwd: no strides");
+    if (dims[0] * (dims[3] + dims[4]) == 0) return MPR_OK;
+    MPR_REQUIRE(dims[3] == 0 || (q && out && lse && dout), "xattn_bwd: null pointer");
+    MPR_REQUIRE(dims[4] == 0 || (k && v), "xattn_bwd: null pointer");
+    MPR_REQUIRE(!dk == !dv, "xattn_bwd: dk and dv are wanted together");
+    const XPlan p = xattn_plan(dims);
+    MPR_REQUIRE(p.bwd_bytes == 0 || (ws && ws_bytes >= p.bwd_bytes),
+                "xattn_bwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
+                (long long)p.bwd_bytes);
+    XArgs a = xattn_args(q, k, v, keep, dims, strides, scale);
+    a.o = out;
+    a.lse = const_cast<float*>(lse);
+    a.dout = dout;
+    a.do_bs = strides[10]; a.do_ls = strides[11]; a.do_hs = strides[12];
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    char* w = static_cast<char*>(ws);
+    a.delta = reinterpret_cast<float*>(w + p.delta);
+    a.part = reinterpret_cast<float*>(w + up256((int64_t)a.B * a.H * a.Lq * 4));
+    a.part2 = reinterpret_cast<float*>(w + p.part2);
+    return by_dtype(dtype, [&](auto z) -> int {
+      return xattn_backward<decltype(z)>(a, p, op_stream(stream));
+    });
+  });
+}
+
+}  // extern "C"

@@ -29,6 +29,7 @@ from torch import nn
 
 from . import _lib
 from .encoders import TOKENS, DeviceViT
+from .ops import clip_grads_
 from .staging import to_device
 from .t5 import DeviceT5
 
@@ -573,6 +574,12 @@ class T5VisionModel(nn.Module):
         loss = self.T5_model(inputs_embeds=combined, attention_mask=mask, labels=labels).loss
         self._flush_hints()  # the next batch's retrieval, beside this T5 forward (hint_next)
         return loss
+
+    def clip_grad_norm_(self, max_norm: float):
+        """Clips the gradients that ``loss.backward()`` left on the parameters to a global L2 norm
+        of ``max_norm``, in place, and returns the norm before it (``ops.clip_grads_``): call it
+        between ``backward()`` and the optimizer's step.  The norm stays on the device."""
+        return clip_grads_([p.grad for p in self.parameters() if p.grad is not None], max_norm)
 
     def _forward_key(self, batch):
         # what prepare_input's result depends on besides the batch: the tied embedding's values

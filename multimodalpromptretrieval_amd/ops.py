@@ -1,0 +1,487 @@
+"""Tensor operators for tuning and serving the T5 reader on the device.
+
+The framework's trainer (``train.py``) runs the reference's own step: fp32, teacher forcing, cross
+entropy.  These operators are for what a user builds next to it — tuning the reader on chosen and
+rejected answers, in bf16, on longer prompts — each a differentiable torch function over
+hand-written kernels of libmpr.so:
+
+* ``embed`` — scaled embedding lookup; its gradient sums the positions of each token, sorted on the
+  device (``train.EmbedFn`` groups them on the host);
+* ``cross_attention`` — attention to an encoder's states of another length, with key / value heads
+  that query heads share, forward and backward, and its form for single tokens;
+* ``sequence_logps`` / ``preference_loss`` — log-probabilities of label sequences, and the loss of
+  paired answers over them, with the gradient of the logits;
+* ``grad_norm`` / ``clip_grads_`` — the global L2 norm of many gradients, and their clipping
+  (``T5VisionModel.clip_grad_norm_`` clips a model's).
+
+Conventions.  Floating tensors are float32, bfloat16 or float16; sums and statistics are 32 bits or
+wider, and a result is rounded once to its type (bf16 attention also rounds the probabilities
+between its two products).  Work goes to the current stream of the tensors' device, which need not
+be the current device.  Workspaces come from torch's caching allocator in every call, so calls on
+several streams and captured graphs share nothing; nothing waits for the GPU, so device tensors may
+be captured into a graph (token ids and labels on the host are uploaded: not inside a capture).
+Results are the same bits on every run.  What a call cannot take is refused with ``ValueError`` /
+``TypeError`` before anything is launched.  The gradients themselves are not differentiable again.
+
+Capturing a backward pass: torch ties a leaf's gradient accumulation to the stream of the first
+graph that reached it, so drop every loss of the same leaves that ran eagerly (``del loss``) before
+capturing, as torch asks for any captured backward.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_IDS = {torch.int32: 0, torch.int64: 1}
+
+
+# ---- arguments -----------------------------------------------------------------------------------
+def _floating(t, name: str) -> int:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name}: a tensor is needed, got {type(t).__name__}")
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name}: float32, bfloat16 or float16 is needed, got {t.dtype}")
+    return code
+
+
+def _on_gpu(t, name: str) -> None:
+    if t.device.type != "cuda":
+        raise ValueError(f"{name}: libmpr runs on a GPU, the tensor is on {t.device}")
+
+
+def _same(a, b, what: str) -> None:
+    if a.device != b.device:
+        raise ValueError(f"{what}: tensors on {a.device} and {b.device}")
+    if a.dtype != b.dtype:
+        raise TypeError(f"{what}: {a.dtype} and {b.dtype}")
+
+
+def _rows(t):
+    """The tensor with its last dimension contiguous."""
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _matrix(t):
+    """A matrix whose rows are contiguous and do not overlap."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _tokens(t, device, name: str, below: int, lowest: int):
+    """Token ids as a contiguous device tensor; ids on the host are checked and uploaded."""
+    if not isinstance(t, torch.Tensor) or t.dtype not in _IDS:
+        raise TypeError(f"{name}: an int32 or int64 tensor is needed, got "
+                        f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if t.device.type == "cpu":
+        if t.numel() and (int(t.max()) >= below or int(t.min()) < lowest):
+            raise IndexError(f"{name}: values from {int(t.min())} to {int(t.max())}, "
+                             f"needed in [{lowest}, {below})")
+    elif t.device != device:
+        raise ValueError(f"{name}: on {t.device}, needed on {device} (or the host)")
+    if device.type != "cuda":
+        raise ValueError(f"{name}: libmpr runs on a GPU, the operands are on {device}")
+    if t.device == device:
+        return t.contiguous()
+    with torch.cuda.device(device):
+        return _lib.to_device_async(t, device).contiguous()
+
+
+def _i64(*vals):
+    return (ctypes.c_int64 * len(vals))(*vals)
+
+
+def _call(device, name: str, *args) -> None:
+    """The library call on the current stream of `device`."""
+    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(device):
+            _lib.call(name, *args, stream)
+
+
+def _workspace(nbytes: int, device):
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+
+
+# ---- embedding -----------------------------------------------------------------------------------
+def _embed_fwd(weight, ids, scale):
+    w = _matrix(weight.detach())
+    V, d = w.shape
+    out = torch.empty((*ids.shape, d), dtype=w.dtype, device=w.device)
+    _call(w.device, "mpr_embed_lookup", _lib.ptr(w), _DTYPES[w.dtype], V, w.stride(0),
+          _lib.ptr(ids), _IDS[ids.dtype], ids.numel(), d, scale, _lib.ptr(out))
+    return out
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.table = (weight.shape, weight.dtype)
+        ctx.args = (scale, padding_idx)
+        return _embed_fwd(weight, ids, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (ids,), ((V, d), dtype), (scale, pad) = ctx.saved_tensors, ctx.table, ctx.args
+        n, code = ids.numel(), _DTYPES[dtype]
+        dout = _matrix(dout.reshape(n, d))
+        dw = torch.empty((V, d), dtype=dtype, device=dout.device)
+        nbytes = ctypes.c_int64()
+        _lib.call("mpr_embed_grad_workspace", code, n, V, d, ctypes.byref(nbytes))
+        ws = _workspace(nbytes.value, dout.device)
+        _call(dout.device, "mpr_embed_grad", _lib.ptr(dout), code, dout.stride(0),
+              _lib.ptr(ids), _IDS[ids.dtype], n, V, d, scale, pad, _lib.ptr(dw), _lib.ptr(ws),
+              nbytes.value)
+        return dw, None, None, None
+
+
+def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
+    """``scale * weight[ids]``: ``weight`` [V, d] -> [*ids.shape, d] in the weight's type.
+
+    The gradient ``dweight[v] = scale * sum of dout over the positions with ids == v`` is dense, and
+    zero for ``padding_idx`` (counted from the end if negative).  ``ids``: int32 or int64, on the
+    weight's device or the host (there checked against the table).  An id outside the table that
+    lies on the device cannot be refused without waiting for the GPU: it gives a row of NaN and no
+    gradient."""
+    _floating(weight, "embed weight")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"embed: a table [V, d] is needed, got {tuple(weight.shape)}")
+    V = weight.shape[0]
+    pad = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise ValueError(f"embed: padding_idx {padding_idx} in a table of {V} rows")
+        pad = int(padding_idx) % V
+    scale = float(scale)
+    ids = _tokens(ids, weight.device, "embed ids", V, 0)
+    if _wants_grad(weight):
+        return _Embed.apply(weight, ids, scale, pad)
+    return _embed_fwd(weight, ids, scale)
+
+
+# ---- cross attention -----------------------------------------------------------------------------
+def _xattn_dims(q, k):
+    B, Lq, H, D = q.shape
+    return _i64(B, H, k.shape[2], Lq, k.shape[1], D)
+
+
+def _xattn_strides(q, k, v, keep, dout=None):
+    s = [*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+         0 if keep is None else keep.stride(0)]
+    return _i64(*s, *(dout.stride()[:3] if dout is not None else (0, 0, 0)))
+
+
+def _xattn_bytes(dims, code):
+    fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
+    _lib.call("mpr_xattn_workspace", dims, code, ctypes.byref(fwd), ctypes.byref(bwd))
+    return fwd.value, bwd.value
+
+
+def _xattn_fwd(q, k, v, keep, scale, want_lse):
+    code, dims = _DTYPES[q.dtype], _xattn_dims(q, k)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = None
+    if want_lse:
+        B, Lq, H, _ = q.shape
+        lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
+    nbytes, _ = _xattn_bytes(dims, code)
+    ws = _workspace(nbytes, q.device)
+    _call(q.device, "mpr_xattn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(keep), code,
+          dims, _xattn_strides(q, k, v, keep), scale, _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws),
+          nbytes)
+    return out, lse
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, keep, scale):
+        q, k, v = (_rows(t.detach()) for t in (q, k, v))
+        out, lse = _xattn_fwd(q, k, v, keep, scale, True)
+        ctx.save_for_backward(q, k, v, keep, out, lse)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, keep, out, lse = ctx.saved_tensors
+        dout = _rows(dout)
+        code, dims = _DTYPES[q.dtype], _xattn_dims(q, k)
+        need_q, need_k, need_v = ctx.needs_input_grad[:3]
+
+        def like(t, wanted):
+            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
+        dq = like(q, need_q)
+        dk, dv = (like(t, need_k or need_v) for t in (k, v))
+        _, nbytes = _xattn_bytes(dims, code)
+        ws = _workspace(nbytes, q.device)
+        _call(q.device, "mpr_xattn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(keep),
+              code, dims, _xattn_strides(q, k, v, keep, dout), ctx.scale, _lib.ptr(out),
+              _lib.ptr(lse), _lib.ptr(dout), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
+              _lib.ptr(ws), nbytes)
+        return dq, dk if need_k else None, dv if need_v else None, None, None
+
+
+def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
+    """``softmax(scale q k^T) v`` of queries ``q`` [B, Lq, H, D] over an encoder's ``k``, ``v``
+    [B, Lk, Hkv, D] -> [B, Lq, H, D].
+
+    H is a multiple of Hkv: query head h reads key head ``h // (H // Hkv)``, and the gradients of a
+    key head sum its query heads'.  D is a multiple of 8 up to 128.  ``scale`` 1 is T5's.
+    ``key_mask`` [B, Lk] (or [1, Lk]): the keys that are not 0 / False are attended to; what a
+    masked key holds (NaN, infinities) touches nothing and its gradient is 0, and a row whose keys
+    are all masked, or Lk = 0, gives 0.  Any strides will do (the halves of a joint k | v
+    projection), but the elements of a head are read in place only if they are adjacent."""
+    _floating(q, "cross_attention q")
+    for t, name in ((k, "k"), (v, "v")):
+        _floating(t, "cross_attention " + name)
+        _same(q, t, "cross_attention q, " + name)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("cross_attention: q [B, Lq, H, D] and k, v [B, Lk, Hkv, D] are needed, "
+                         f"got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, Lk, Hkv, D = k.shape
+    H = q.shape[2]
+    if q.shape[0] != B or q.shape[3] != D or Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"cross_attention: q {tuple(q.shape)} does not fit k {tuple(k.shape)} "
+                         "(batch and head dim equal, query heads a multiple of key heads)")
+    if D < 8 or D > 128 or D % 8:
+        raise ValueError(f"cross_attention: head dim {D} (a multiple of 8 up to 128)")
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"cross_attention: scale {scale}")
+    keep = None
+    if key_mask is not None:
+        if not isinstance(key_mask, torch.Tensor):
+            raise TypeError("cross_attention: key_mask is a tensor")
+        if key_mask.device != q.device:
+            raise ValueError(f"cross_attention: key_mask on {key_mask.device}, q on {q.device}")
+        if key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Lk:
+            raise ValueError(f"cross_attention: key_mask {tuple(key_mask.shape)}, "
+                             f"needed [{B}, {Lk}]")
+    _on_gpu(q, "cross_attention")
+    if key_mask is not None:
+        keep = key_mask if key_mask.dtype == torch.bool else key_mask != 0
+        keep = _rows(keep.detach().expand(B, Lk)).view(torch.uint8)
+    if _wants_grad(q, k, v):
+        return _CrossAttention.apply(q, k, v, keep, scale)
+    return _xattn_fwd(_rows(q.detach()), _rows(k.detach()), _rows(v.detach()), keep, scale,
+                      False)[0]
+
+
+# ---- log-probabilities and the preference loss -----------------------------------------------------
+def _logps_shapes(logits, labels, what):
+    _floating(logits, what + " logits")
+    if logits.dim() != 3 or logits.shape[2] < 1:
+        raise ValueError(f"{what}: logits [S, T, V] are needed, got {tuple(logits.shape)}")
+    S, T, V = logits.shape
+    if not isinstance(labels, torch.Tensor) or tuple(labels.shape) != (S, T):
+        raise ValueError(f"{what}: labels [{S}, {T}] are needed, got "
+                         f"{tuple(labels.shape) if isinstance(labels, torch.Tensor) else labels}")
+
+
+def _label_ids(logits, labels, what):
+    return _tokens(labels, logits.device, what + " labels", logits.shape[2], -2 ** 63)
+
+
+def _logps_fwd(logits, labels, pair):
+    """(logps, row_stat, loss, dlogps); pair: (ref, beta, label_smoothing) or None."""
+    S, T, V = logits.shape
+    dev = logits.device
+
+    def f32(*shape):
+        return torch.empty(shape, dtype=torch.float32, device=dev)
+    logps, stat = f32(S), f32(S, T, 2)
+    loss, dlogps = (f32(), f32(S)) if pair else (None, None)
+    ref, beta, smooth = pair or (None, 0.0, 0.0)
+    nbytes = ctypes.c_int64()
+    _lib.call("mpr_logps_workspace", S, T, V, ctypes.byref(nbytes))
+    ws = _workspace(nbytes.value, dev)
+    _call(dev, "mpr_logps_fwd", _lib.ptr(logits), _DTYPES[logits.dtype], S, T, V,
+          logits.stride(0), logits.stride(1), _lib.ptr(labels), _IDS[labels.dtype], T,
+          _lib.ptr(logps), _lib.ptr(stat), _lib.ptr(ref), beta, smooth, _lib.ptr(loss),
+          _lib.ptr(dlogps), _lib.ptr(ws), nbytes.value)
+    return logps, stat, loss, dlogps
+
+
+def _logps_bwd(logits, labels, stat, dlogps, mult):
+    S, T, V = logits.shape
+    dx = torch.empty((S, T, V), dtype=logits.dtype, device=logits.device)
+    _call(logits.device, "mpr_logps_bwd", _lib.ptr(logits), _DTYPES[logits.dtype], S, T, V,
+          logits.stride(0), logits.stride(1), _lib.ptr(labels), _IDS[labels.dtype], T,
+          _lib.ptr(stat), _lib.ptr(dlogps), _lib.ptr(mult), _lib.ptr(dx))
+    return dx
+
+
+class _SequenceLogps(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels):
+        logits = _rows(logits.detach())
+        logps, stat, _, _ = _logps_fwd(logits, labels, None)
+        ctx.save_for_backward(logits, labels, stat)
+        return logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogps):
+        logits, labels, stat = ctx.saved_tensors
+        return _logps_bwd(logits, labels, stat, dlogps.contiguous(), None), None
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ref, beta, smooth):
+        logits = _rows(logits.detach())
+        logps, stat, loss, dlogps = _logps_fwd(logits, labels, (ref, beta, smooth))
+        ctx.save_for_backward(logits, labels, stat, dlogps)
+        ctx.mark_non_differentiable(logps)
+        return loss, logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _):
+        logits, labels, stat, dlogps = ctx.saved_tensors
+        return (_logps_bwd(logits, labels, stat, dlogps, dloss.contiguous()), None, None, None,
+                None)
+
+
+def sequence_logps(logits, labels):
+    """``sum_t log_softmax(logits[s, t])[labels[s, t]]`` over the positions whose label is not
+    negative (-100: ignored, as the trainer's loss does): ``logits`` [S, T, V], ``labels`` [S, T]
+    (int32 or int64, device or host) -> [S] float32.
+
+    The rows of ignored positions are not read, and their gradient is 0.  A label >= V on the
+    device gives NaN (on the host: IndexError).  Under ``no_grad`` this is the reference model's
+    side of ``preference_loss``."""
+    _logps_shapes(logits, labels, "sequence_logps")
+    labels = _label_ids(logits, labels, "sequence_logps")
+    if _wants_grad(logits):
+        return _SequenceLogps.apply(logits, labels)
+    return _logps_fwd(_rows(logits.detach()), labels, None)[0]
+
+
+def preference_loss(logits, labels, ref_logps, beta: float = 0.1, label_smoothing: float = 0.0):
+    """The preference loss of P answer pairs: (loss, logps).
+
+    ``logits`` [2P, T, V], ``labels`` [2P, T] (negative: ignored) and ``ref_logps`` [2P], the
+    reference model's ``sequence_logps``, hold the chosen answers first, then the rejected ones in
+    the same order.  ``margin_p = beta ((logps[p] - logps[P + p]) - (ref[p] - ref[P + p]))`` and
+    ``loss = mean_p -(1 - label_smoothing) log sigmoid(margin_p) - label_smoothing log
+    sigmoid(-margin_p)``.  ``loss`` (a float32 scalar) is differentiable by ``logits``; ``logps``
+    [2P] (float32) is for the metrics and is not."""
+    _logps_shapes(logits, labels, "preference_loss")
+    S = logits.shape[0]
+    if S == 0 or S % 2:
+        raise ValueError(f"preference_loss: {S} sequences are not pairs")
+    if not isinstance(ref_logps, torch.Tensor) or tuple(ref_logps.shape) != (S,):
+        raise ValueError(f"preference_loss: ref_logps [{S}] are needed")
+    if ref_logps.device != logits.device:
+        raise ValueError(f"preference_loss: ref_logps on {ref_logps.device}, logits on "
+                         f"{logits.device}")
+    beta, smooth = float(beta), float(label_smoothing)
+    if not math.isfinite(beta):
+        raise ValueError(f"preference_loss: beta {beta}")
+    if not 0.0 <= smooth <= 0.5:
+        raise ValueError(f"preference_loss: label_smoothing {smooth} (0 to 0.5)")
+    labels = _label_ids(logits, labels, "preference_loss")
+    ref = ref_logps.detach().to(torch.float32).contiguous()
+    if _wants_grad(logits):
+        return _PreferenceLoss.apply(logits, labels, ref, beta, smooth)
+    logps, _, loss, _ = _logps_fwd(_rows(logits.detach()), labels, (ref, beta, smooth))
+    return loss, logps
+
+
+# ---- gradient clipping ---------------------------------------------------------------------------
+def _dense(t) -> bool:
+    """Whether the tensor fills its memory without gaps or repeats (in whatever order)."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for n, s in sorted(zip(t.shape, t.stride()), key=lambda p: p[1]):
+        if n != 1:
+            if s != want:
+                return False
+            want *= n
+    return True
+
+
+def _clip(grads, out, max_norm, eps, what):
+    grads = list(grads)
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"{what}: {len(grads)} gradients and {len(out)} outputs")
+    desc = (ctypes.c_int64 * (5 * len(grads)))()
+    device = None
+    for i, g in enumerate(grads):
+        code = _floating(g, f"{what} gradient {i}")
+        device = device or g.device
+        if g.device != device or g.layout is not torch.strided:
+            raise ValueError(f"{what}: gradient {i} is a {g.layout} tensor on {g.device}, needed "
+                             f"dense on {device}")
+        if not _dense(g):
+            raise ValueError(f"{what}: gradient {i} {tuple(g.shape)} with strides {g.stride()} "
+                             "leaves gaps in its memory (clip a .contiguous() copy)")
+        o = 5 * i
+        desc[o], desc[o + 1], desc[o + 2] = g.data_ptr(), g.numel(), code
+        if max_norm is None:
+            continue
+        if out is None:
+            desc[o + 3], desc[o + 4] = desc[o], code
+            continue
+        t = out[i]
+        desc[o + 4] = _floating(t, f"{what} output {i}")
+        if t.device != device or t.shape != g.shape:
+            raise ValueError(f"{what}: output {i} is {tuple(t.shape)} on {t.device}, its gradient "
+                             f"{tuple(g.shape)} on {device}")
+        if t.stride() != g.stride() and not (t.is_contiguous() and g.is_contiguous()):
+            raise ValueError(f"{what}: output {i} is laid out otherwise than its gradient")
+        desc[o + 3] = t.data_ptr()
+    if device is None:
+        return torch.zeros(())
+    _on_gpu(grads[0], what)
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    nbytes = ctypes.c_int64()
+    _lib.call("mpr_clip_workspace", len(grads), desc, ctypes.byref(nbytes))
+    ws = _workspace(nbytes.value, device)
+    _call(device, "mpr_clip_grads", len(grads), desc, max_norm or 0.0, eps, _lib.ptr(norm),
+          _lib.ptr(ws), nbytes.value)
+    return norm
+
+
+@torch.no_grad()
+def grad_norm(grads):
+    """The L2 norm of all values of the tensors together (a float32 scalar on their device; 0 on the
+    host for none).  Squares are summed in 64 bits."""
+    return _clip(grads, None, None, 0.0, "grad_norm")
+
+
+@torch.no_grad()
+def clip_grads_(grads, max_norm: float, eps: float = 1e-6, out=None):
+    """Scales the gradients by ``min(1, max_norm / (norm + eps))`` and returns ``norm``, their
+    global L2 norm before it (``grad_norm``).
+
+    In place, or into ``out``: a tensor for each gradient, of its shape and any floating type (the
+    optimizer's fp32 buffer for bf16 gradients).  Gradients below the limit are not written in
+    place at all.  The types may differ between tensors.  A norm that is not finite goes through as
+    it is: NaN makes every gradient NaN, infinity makes finite ones 0.  Tensors that share memory
+    (one gradient listed twice) and gradients with gaps in their memory are refused."""
+    max_norm, eps = float(max_norm), float(eps)
+    if not max_norm >= 0.0 or not eps >= 0.0:
+        raise ValueError(f"clip_grads_: max_norm {max_norm}, eps {eps}")
+    grads = list(grads)
+    out = None if out is None else list(out)
+    norm = _clip(grads, out, max_norm, eps, "clip_grads_")
+    if grads:
+        torch.autograd.graph.increment_version(grads if out is None else out)
+    return norm

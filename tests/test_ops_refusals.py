@@ -1,0 +1,190 @@
+"""What the tensor operators of ``ops.py`` and their C entries refuse, before anything reaches a GPU
+(no GPU needed: every call here ends in an error, or in a size computed on the host)."""
+import ctypes
+
+import pytest
+import torch
+
+from multimodalpromptretrieval_amd import _lib, ops
+
+T = torch.zeros
+
+
+def test_embed_refusals():
+    w, ids = T(5, 4), T(3, dtype=torch.int64)
+    for bad in (T(5), T(0, 4), T(5, 0), T(2, 3, 4)):
+        with pytest.raises(ValueError, match="table"):
+            ops.embed(bad, ids)
+    with pytest.raises(TypeError):
+        ops.embed(w.double(), ids)
+    with pytest.raises(TypeError):
+        ops.embed([1.0], ids)
+    for pad in (5, -6):
+        with pytest.raises(ValueError, match="padding_idx"):
+            ops.embed(w, ids, padding_idx=pad)
+    for bad in (ids.float(), ids.short(), [0, 1]):
+        with pytest.raises(TypeError, match="int32 or int64"):
+            ops.embed(w, bad)
+    for bad in (ids + 5, ids - 1):
+        with pytest.raises(IndexError):
+            ops.embed(w, bad)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.embed(w, ids)
+
+
+def test_cross_attention_refusals():
+    q, k = T(2, 3, 4, 64), T(2, 5, 2, 64)
+    for a, b, c in ((q[0], k, k), (q, k[0], k[0]), (q, k, k[:, :4]), (q[:1], k, k),
+                    (q[..., :32], k, k), (q[:, :, :3], k, k), (q[:, :, :0], k, k),
+                    (q, k[:, :, :0], k[:, :, :0])):
+        with pytest.raises(ValueError):
+            ops.cross_attention(a, b, c)
+    for D in (4, 12, 136, 256):
+        with pytest.raises(ValueError, match="head dim"):
+            ops.cross_attention(T(1, 1, 1, D), T(1, 2, 1, D), T(1, 2, 1, D))
+    with pytest.raises(TypeError):
+        ops.cross_attention(q, k.half(), k.half())
+    with pytest.raises(TypeError):
+        ops.cross_attention(q, k, k.bfloat16())
+    with pytest.raises(TypeError):
+        ops.cross_attention(*(t.double() for t in (q, k, k)))
+    for m in (T(2, 4), T(3, 5), T(5), T(2, 1, 1, 5), T(2, 1)):
+        with pytest.raises(ValueError, match="key_mask"):
+            ops.cross_attention(q, k, k, m)
+    with pytest.raises(TypeError, match="key_mask"):
+        ops.cross_attention(q, k, k, [[1] * 5] * 2)
+    for s in (float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            ops.cross_attention(q, k, k, scale=s)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.cross_attention(q, k, k)
+
+
+def test_preference_refusals():
+    x, y, r = T(4, 3, 7), T(4, 3, dtype=torch.int64), T(4)
+    for fn in (lambda a, b: ops.sequence_logps(a, b), lambda a, b: ops.preference_loss(a, b, r)):
+        for bad in (x[0], T(4, 3, 0)):
+            with pytest.raises(ValueError, match="logits"):
+                fn(bad, y)
+        for bad in (y[:, :2], y[0], None):
+            with pytest.raises(ValueError, match="labels"):
+                fn(x, bad)
+        with pytest.raises(TypeError):
+            fn(x.double(), y)
+        with pytest.raises(TypeError):
+            fn(x, y.float())
+        with pytest.raises(IndexError):
+            fn(x, y + 7)
+        with pytest.raises(ValueError, match="GPU"):
+            fn(x, y - 100)
+    for n in (0, 3):
+        with pytest.raises(ValueError, match="pairs"):
+            ops.preference_loss(x[:n], y[:n], r[:n])
+    for bad in (r[:3], r[:, None], 0.0):
+        with pytest.raises(ValueError, match="ref_logps"):
+            ops.preference_loss(x, y, bad)
+    for kw in (dict(beta=float("nan")), dict(beta=float("inf")), dict(label_smoothing=-0.1),
+               dict(label_smoothing=0.6), dict(label_smoothing=float("nan"))):
+        with pytest.raises(ValueError):
+            ops.preference_loss(x, y, r, **kw)
+
+
+def test_clip_refusals():
+    g = T(4, 6)
+    for kw in (dict(max_norm=-1.0), dict(max_norm=float("nan")), dict(max_norm=1.0, eps=-1.0)):
+        with pytest.raises(ValueError):
+            ops.clip_grads_([g], **kw)
+    with pytest.raises(TypeError):
+        ops.clip_grads_([g.double()], 1.0)
+    with pytest.raises(TypeError):
+        ops.grad_norm([1.0])
+    with pytest.raises(ValueError, match="gaps"):
+        ops.grad_norm([g[:, ::2]])
+    with pytest.raises(ValueError, match="gaps"):
+        ops.grad_norm([g[:, :1].expand(4, 6)])
+    with pytest.raises(ValueError, match="outputs"):
+        ops.clip_grads_([g], 1.0, out=[])
+    with pytest.raises(ValueError, match="output 0"):
+        ops.clip_grads_([g], 1.0, out=[T(4, 5)])
+    with pytest.raises(ValueError, match="laid out"):
+        ops.clip_grads_([g], 1.0, out=[T(6, 4).t()])
+    with pytest.raises(ValueError, match="GPU"):
+        ops.clip_grads_([g], 1.0)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.grad_norm([g.t()])
+    assert float(ops.grad_norm([])) == 0.0
+
+
+def refused(name, *args):
+    with pytest.raises(RuntimeError, match=name.replace("mpr_", "")):
+        _lib.call(name, *args)
+
+
+def i64(*v):
+    return (ctypes.c_int64 * len(v))(*v)
+
+
+P = ctypes.c_void_p(4096)  # a pointer that no refused call follows
+
+
+def test_c_entries_refuse_bad_arguments():
+    n = ctypes.c_int64()
+    out = ctypes.byref(n)
+    for dtype, ids, V, d in ((3, 1, 5, 4), (0, -1, 5, 4), (0, 1 << 31, 5, 4), (0, 1, 0, 4),
+                             (0, 1, 1 << 31, 4), (0, 1, 5, 0)):
+        refused("mpr_embed_grad_workspace", dtype, ids, V, d, out)
+        refused("mpr_embed_lookup", P, dtype, V, d, P, 1, ids, d, 1.0, P, None)
+    refused("mpr_embed_lookup", P, 0, 5, 3, P, 1, 2, 4, 1.0, P, None)  # rows overlap
+    refused("mpr_embed_lookup", None, 0, 5, 4, P, 1, 2, 4, 1.0, P, None)
+    refused("mpr_embed_grad", P, 0, 4, P, 1, 9, 5, 4, 1.0, -1, P, P, 16, None)  # workspace
+    refused("mpr_embed_grad", P, 0, 4, P, 1, 9, 5, 4, 1.0, -1, None, P, 1 << 40, None)
+    good = (2, 4, 2, 3, 5, 64)
+    for i, v in ((0, -1), (1, 3), (1, 0), (2, 0), (3, -1), (3, 1 << 31), (4, 1 << 31), (5, 4),
+                 (5, 136), (5, 20)):
+        dims = i64(*(v if j == i else x for j, x in enumerate(good)))
+        refused("mpr_xattn_workspace", dims, 0, out, out)
+    refused("mpr_xattn_workspace", None, 0, out, out)
+    refused("mpr_xattn_workspace", i64(*good), 7, out, out)
+    st = i64(*[64] * 13)
+    refused("mpr_xattn_fwd", None, P, P, None, 0, i64(*good), st, 1.0, P, P, None, 0, None)
+    refused("mpr_xattn_fwd", P, P, P, None, 0, i64(*good), None, 1.0, P, P, None, 0, None)
+    refused("mpr_xattn_bwd", P, P, P, None, 0, i64(*good), st, 1.0, P, None, P, P, P, P, P,
+            1 << 40, None)
+    refused("mpr_xattn_bwd", P, P, P, None, 0, i64(*good), st, 1.0, P, P, P, P, P, None, P,
+            1 << 40, None)
+    refused("mpr_xattn_bwd", P, P, P, None, 0, i64(*good), st, 1.0, P, P, P, P, P, P, P, 8, None)
+    refused("mpr_logps_workspace", 2, 3, 0, out)
+    refused("mpr_logps_workspace", 1 << 20, 1 << 20, 5, out)
+    refused("mpr_logps_workspace", 2, 3, 4, None)
+
+    def logps(dtype=0, S=2, T=3, V=4, logits=P, ref=P, loss=P, ws=1 << 40):
+        refused("mpr_logps_fwd", logits, dtype, S, T, V, 12, 4, P, 1, 3, P, P, ref, 0.1, 0.0, loss,
+                P, P, ws, None)
+    logps(dtype=5)
+    logps(S=-1)
+    logps(S=3)  # a loss of three sequences
+    logps(ref=None)
+    logps(logits=None)
+    logps(ws=8)
+    refused("mpr_logps_bwd", P, 0, 2, 3, 4, 12, 4, P, 1, 3, P, None, None, P, None)
+    a = 1 << 20
+    for desc in ((a, -1, 0, a, 0), (a, 4, 3, a, 3), (0, 4, 0, a, 0), (a, 4, 0, a, 1),
+                 (a, 4, 0, a + 4, 0), (a, 4, 0, a, 0, a + 8, 4, 0, a + 8, 0),
+                 (a, 4, 0, a, 0, a + 64, 4, 0, 0, 0), (a, 4, 0, a + 64, 0, a + 128, 4, 0, a + 72, 0)):
+        refused("mpr_clip_grads", len(desc) // 5, i64(*desc), 1.0, 0.0, P, P, 1 << 40, None)
+    refused("mpr_clip_grads", 1, i64(a, 4, 0, a, 0), 1.0, 0.0, None, P, 1 << 40, None)
+    refused("mpr_clip_grads", 1, i64(a, 4, 0, a, 0), 1.0, 0.0, P, P, 8, None)
+    refused("mpr_clip_grads", 1, None, 1.0, 0.0, P, P, 1 << 40, None)
+
+
+def test_workspaces_grow_with_the_work():
+    n = ctypes.c_int64()
+    sizes = []
+    for ids in (0, 1, 5000, 1 << 20):
+        _lib.call("mpr_embed_grad_workspace", 1, ids, 32128, 768, ctypes.byref(n))
+        sizes.append(n.value)
+    assert sizes[0] == 0 and sizes == sorted(sizes)
+    fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
+    _lib.call("mpr_xattn_workspace", i64(4, 16, 4, 1024, 4096, 128), 1, ctypes.byref(fwd),
+              ctypes.byref(bwd))
+    assert bwd.value >= 4 * 16 * 1024 * 4
