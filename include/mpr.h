@@ -429,7 +429,7 @@ int mpr_embed_bwd(const float* dY, int32_t d, const int32_t* uniq, const int32_t
  *   the order of the positions.
  *   mpr_xattn_fwd / _bwd: attention of q [B, Lq, H, D] over k, v [B, Lk, Hkv, D], H a multiple of
  *   Hkv, D a multiple of 8 up to 128, elements of a head contiguous; keep [B, Lk] bytes (0: the key
- *   counts for nothing, whatever it holds) or NULL.  dims = {B, H, Hkv, Lq, Lk, D}; strides (in
+ *   counts for nothing, whatever it holds) or NULL.  scale >= 0.  dims = {B, H, Hkv, Lq, Lk, D}; strides (in
  *   elements) = {q batch, position, head, k .., v .., keep batch, dout batch, position, head (bwd
  *   only)}.  out [B, Lq, H, D], lse [B, H, Lq] (base-2 log of the rows' sums; may be NULL in a
  *   forward alone), dq as out (NULL: not wanted), dk / dv [B, Lk, Hkv, D] (both or none), all

@@ -40,8 +40,11 @@ struct XArgs {
   int64_t q_bs, q_ls, q_hs, k_bs, k_ls, k_hs, v_bs, v_ls, v_hs, keep_bs, do_bs, do_ls, do_hs;
   int B, H, Hkv, G, Lq, Lk, D;
   int R;             // rows of a key head: G Lq
+  uint64_t lq_mul;   // r / Lq = r lq_mul >> lq_shift for r < 2^30
+  int lq_shift;
   int tiles, splits, per_split;  // blocks along the tiled axis, and shares of the other one
-  float c;           // scale log2(e)
+  float c;           // scale log2(e), above 0
+  float slack;       // how far scores may pass the running maximum: 8 / c
   float scale;
   void* out;         // forward: [B, Lq, H, D]
   float* lse;        // [B, H, Lq]: max + log2(sum) of the scaled scores in base 2
@@ -54,26 +57,31 @@ struct XArgs {
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // ---- the two matrix cores ------------------------------------------------------------------------
-// A chunk is the contraction of one call; frag: a lane's share of it.  Lane l holds index l & 31 of
-// the operand's own axis; its half h = l >> 5 of the contraction.
-//   row(p, ld, ...): operand rows lie as rows of LDS, the contraction along them
-//   col(p, ld, ...): the contraction runs over rows of LDS, in the order in which a product's result
-//                    holds its rows: result register r of half h is row 8 (r / 4) + 4 h + r % 4
+// LDS tiles hold rows of DP elements in 16-byte pieces; piece c of row r lies at piece c ^ swz(r):
+// eight rows of one piece, and four rows of two neighbouring pieces, then cover all the banks, which
+// is what a row read and a column read ask for at a time.
+__device__ __forceinline__ int swz(int r) { return ((r & 3) << 1) | ((r >> 2) & 1); }
+
+// A chunk is the contraction of one call (two pieces); frag: a lane's share of it.  Lane l holds
+// index l & 31 of the operand's own axis; its half h = l >> 5 of the contraction.
+//   row(p, r0, c): operand rows r0 .. r0 + 31 lie as rows of LDS, chunk c of their columns
+//   col(p, k0, m0): the contraction runs over rows k0 .. of LDS, in the order in which a product's
+//                   result holds its rows (result register r of half h is row 8 (r / 4) + 4 h +
+//                   r % 4); the operand's own axis is the columns m0 .. m0 + 31
 struct MmaBf16 {
   typedef bf16 elem;
   typedef bf16x8 frag;
-  static constexpr int CHUNK = 16;  // contraction of a chunk
-  static constexpr int PAD = 8;     // elements between LDS rows: row and column reads spread banks
-  static __device__ __forceinline__ frag row(const elem* p, int ld, int r0, int c0, int lane) {
-    return *reinterpret_cast<const frag*>(p + (r0 + (lane & 31)) * ld + c0 + 8 * (lane >> 5));
-  }
+  static constexpr int CHUNK = 16;
   // ds_read_tr16_b64: 16 lanes read 4 rows of 16 elements and each gets a column of them
-  static __device__ __forceinline__ frag col(const elem* p, int ld, int k0, int m0, int lane) {
+  template <int DP>
+  static __device__ __forceinline__ frag col(const elem* p, int k0, int m0, int lane) {
     const int i = lane & 15, g = lane >> 4;
-    const elem* a = p + (k0 + 4 * (g >> 1) + (i >> 2)) * ld + m0 + 16 * (g & 1) + 4 * (i & 3);
+    const int r = 4 * (g >> 1) + (i >> 2);  // (k0 is a multiple of 8: it does not enter swz)
+    const int sw = (2 * (g & 1) + ((i & 3) >> 1)) ^ swz(r), m8 = m0 >> 3;
+    const elem* a = p + r * DP + ((sw ^ (m8 & 7)) << 3) + 4 * (i & 1) + k0 * DP + ((m8 & ~7) << 3);
     typedef __attribute__((address_space(3))) s16x4* lds4;
     const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)a);
-    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(a + 8 * ld));
+    const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(a + 8 * DP));
     const s16x8 z = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     return __builtin_bit_cast(frag, z);
   }
@@ -92,13 +100,14 @@ struct MmaF32 {
   typedef float elem;
   typedef f32x4 frag;
   static constexpr int CHUNK = 8;
-  static constexpr int PAD = 4;
-  static __device__ __forceinline__ frag row(const elem* p, int ld, int r0, int c0, int lane) {
-    return *reinterpret_cast<const frag*>(p + (r0 + (lane & 31)) * ld + c0 + 4 * (lane >> 5));
-  }
-  static __device__ __forceinline__ frag col(const elem* p, int ld, int k0, int m0, int lane) {
-    const elem* a = p + (k0 + 4 * (lane >> 5)) * ld + m0 + (lane & 31);
-    return frag{a[0], a[ld], a[2 * ld], a[3 * ld]};
+  template <int DP>
+  static __device__ __forceinline__ frag col(const elem* p, int k0, int m0, int lane) {
+    const int h = lane >> 5, x = ((lane & 31) >> 2) ^ h;  // m0 is a multiple of 32: 8 pieces
+    const elem* a = p + 4 * h * DP + (lane & 3);
+    frag f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = a[((x ^ (2 * j)) << 2) + (k0 + j) * DP + m0];
+    return f;
   }
   static __device__ __forceinline__ frag pack(const f32x16& x, int c) {
     return frag{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
@@ -111,35 +120,64 @@ struct MmaF32 {
   }
 };
 
+template <class M>
+constexpr int PIECE = 16 / (int)sizeof(typename M::elem);  // elements
+
+template <class M, int DP>
+__device__ __forceinline__ typename M::frag row_frag(const typename M::elem* p, int r0, int c,
+                                                     int lane) {
+  const int r = lane & 31, x = (lane >> 5) ^ swz(r);
+  return *reinterpret_cast<const typename M::frag*>(
+      p + r * DP + (x ^ (2 * c & 7)) * PIECE<M> + r0 * DP + (2 * c & ~7) * PIECE<M>);
+}
+
 // the row (0 .. 31) that result register r of this lane's half holds
 __device__ __forceinline__ int acc_row(int r, int lane) {
   return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
 }
 
-// ---- staging -------------------------------------------------------------------------------------
-// rows [r0, r0 + n) of a matrix of `rows` rows into LDS as M's elements; rows outside, rows that
-// `keep` drops and columns past D become zeros.  at(r): the row's first element.
-template <class T, class M, int DP, class At>
-__device__ __forceinline__ void stage(typename M::elem* lds, int n, int64_t r0, int64_t rows,
-                                      int D, const uint8_t* keep, At at, int t, int threads) {
-  typedef typename M::elem E;
-  constexpr int N = 8, CH = DP / N, LD = DP + M::PAD;
-  for (int i = t; i < n * CH; i += threads) {
-    const int r = i / CH, c = (i % CH) * N;
-    E x[N];
-#pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = (E)0.f;
-    if (r0 + r < rows && c < D && (!keep || keep[r0 + r])) {
-      const typename Vec<T, N>::type v =
-          *reinterpret_cast<const typename Vec<T, N>::type*>(at(r0 + r) + c);
-#pragma unroll
-      for (int e = 0; e < N; ++e) x[e] = (E)v[e];
-    }
-    E* o = lds + r * LD + c;
-#pragma unroll
-    for (int e = 0; e < N; ++e) o[e] = x[e];
-  }
+// a value's pair in the other half of the wave: f(own, other's) in both
+template <class F>
+__device__ __forceinline__ float halves(float x, F f) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
+
+// ---- staging -------------------------------------------------------------------------------------
+// A tile of ROWS rows on its way from memory to LDS: load() starts the reads of rows [r0, r0 +
+// ROWS) (those past `end` and columns past D read nothing), put() writes them as M's elements, zeros
+// in place of what was not read and of rows whose bit in `words` is 0.  at(r): the row's first
+// element.  Loads are issued a tile ahead and wait in registers while the tile before is computed.
+template <class T, class M, int DP, int ROWS, int THREADS>
+struct Stage {
+  typedef typename M::elem E;
+  static constexpr int N = PIECE<M>, CH = DP / N, CNT = ROWS * CH / THREADS;
+  static_assert(ROWS * CH % THREADS == 0, "whole pieces a thread");
+  typename Vec<T, N>::type x[CNT];
+  template <class At>
+  __device__ __forceinline__ void load(int64_t r0, int64_t end, int D, At at, int t) {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int p = i * THREADS + t, r = p / CH, c = (p % CH) * N;
+      x[i] = typename Vec<T, N>::type{};
+      if (r0 + r < end && c < D)
+        x[i] = *reinterpret_cast<const typename Vec<T, N>::type*>(at(r0 + r) + c);
+    }
+  }
+  __device__ __forceinline__ void put(E* lds, const uint32_t* words, int t) {
+    typedef E piece __attribute__((ext_vector_type(N)));
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) {
+      const int p = i * THREADS + t, r = p / CH, c = p % CH;
+      const bool on = !words || (words[r >> 5] >> (r & 31)) & 1;
+      piece v;
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[e] = on ? (E)x[i][e] : (E)0.f;
+      *reinterpret_cast<piece*>(lds + r * DP + ((c ^ swz(r)) * N)) = v;
+    }
+  }
+};
 
 // a wave's 32 rows as second operands in registers: frag c = contraction chunk c of row lane & 31
 template <class T, class M, int DP>
@@ -160,13 +198,33 @@ __device__ __forceinline__ void load_rows(typename M::frag (&f)[DP / M::CHUNK], 
   }
 }
 
-// bit i: key k0 + i exists and is kept (32 keys)
-__device__ __forceinline__ uint32_t keep_bits(const uint8_t* keep, int64_t k0, int Lk, int lane) {
-  const int64_t k = k0 + (lane & 31);
-  return (uint32_t)__ballot(k < Lk && (!keep || keep[k]));
+// The keys of a block in spans of SPAN: words[i] has a bit for each of the 32 keys from k0 + 32 i
+// that exists (k < end) and that the mask keeps.  Whole tiles without one are passed over.
+constexpr int SPAN = 4096, SPAN_UNIT = 128;  // SPAN_UNIT: a multiple of every tile
+__device__ __forceinline__ void span_words(uint32_t* words, const uint8_t* keep, int64_t k0,
+                                           int64_t end, int t, int threads) {
+  const int n = (int)min((int64_t)SPAN, (end - k0 + SPAN_UNIT - 1) / SPAN_UNIT * SPAN_UNIT);
+  for (int i = t; i < n; i += threads) {  // n and threads are multiples of 64: whole waves
+    const int64_t k = k0 + i;
+    const uint64_t on = __ballot(k < end && (!keep || keep[k]));
+    if ((t & 63) == 0) {
+      words[i >> 5] = (uint32_t)on;
+      words[(i >> 5) + 1] = (uint32_t)(on >> 32);
+    }
+  }
+}
+template <int KT>
+__device__ __forceinline__ int next_tile(const uint32_t* words, int at, int last) {
+  for (; at < last; at += KT) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int u = 0; u < KT / 32; ++u) any |= words[at / 32 + u];
+    if (any) break;
+  }
+  return at;
 }
 
-// [tile | DP x 32 result, transposed] -> rows of 4-element runs: f(d, 4 values)
+// [DP x 32 result, transposed] -> rows of 4-element runs: f(d, 4 values)
 template <int DP, class F>
 __device__ __forceinline__ void for_runs(const f32x16 (&acc)[DP / 32], int lane, F f) {
 #pragma unroll
@@ -178,113 +236,223 @@ __device__ __forceinline__ void for_runs(const f32x16 (&acc)[DP / 32], int lane,
     }
 }
 
+// A wave's accumulator to LDS and back (another wave's, lane for lane)
+template <int NT>
+__device__ __forceinline__ void acc_out(float* lds, const f32x16 (&acc)[NT], int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(lds + ((t * 4 + r) * 64 + lane) * 4) =
+          f32x4{acc[t][4 * r], acc[t][4 * r + 1], acc[t][4 * r + 2], acc[t][4 * r + 3]};
+}
+template <int NT>
+__device__ __forceinline__ void acc_join(const float* lds, f32x16 (&acc)[NT], float own,
+                                         float other, int lane) {
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(lds + ((t * 4 + r) * 64 + lane) * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[t][4 * r + e] = acc[t][4 * r + e] * own + x[e] * other;
+    }
+}
+
 struct RowAt {  // row r of (b, key head): its query head and position
   int h, i;
 };
 __device__ __forceinline__ RowAt row_at(const XArgs& a, int hk, int r) {
-  const int g = r / a.Lq;
+  const int g = (int)((uint64_t)(uint32_t)r * a.lq_mul >> a.lq_shift);
   return {hk * a.G + g, r - g * a.Lq};
 }
 
+// Which (tile, split, batch, key head) a block computes.  Blocks go round robin over the 8 XCDs, so
+// neighbours in the order below, which read the same keys, are given to one XCD and its L2.
+struct Job {
+  int tile, split, b, hk;
+  int64_t bh;
+};
+__device__ __forceinline__ Job job_of(const XArgs& a) {
+  const uint32_t n = gridDim.x, x = blockIdx.x % 8, q = n / 8, r = n % 8;
+  const uint32_t id = x * q + min(x, r) + blockIdx.x / 8;
+  Job j;
+  j.tile = id % a.tiles;
+  const uint32_t rest = id / a.tiles;
+  j.split = rest % a.splits;
+  j.bh = rest / a.splits;
+  j.b = (int)(j.bh / a.Hkv);
+  j.hk = (int)(j.bh % a.Hkv);
+  return j;
+}
+
+constexpr int NW = 4;  // waves of a block
+// Waves a SIMD is to hold (what the registers are shared by).
+template <class M, int DP>
+constexpr int FWD_OCC = sizeof(typename M::elem) == 2 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 2 : 1);
+template <class M, int DP>
+constexpr int BWD_OCC = sizeof(typename M::elem) == 2 && DP == 64 ? 2 : 1;
+// The block's waves: WR of them along the rows (32 each), NW / WR along the staged keys.
+// KT keys are staged at a time.
+template <class M, int WR>
+constexpr int FWD_KT = sizeof(typename M::elem) == 2 ? (WR == 4 ? 64 : 128) : 32 * (NW / WR);
+
 // ---- forward -------------------------------------------------------------------------------------
-// A wave per 32 rows, the block's waves share the staged keys.
-template <class T, class M, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW) void xattn_fwd_kernel(XArgs a) {
+// The running maximum follows the scores only when they pass it by more than 8 (in base 2): until
+// then exponentials up to 2^8 share the old base, and the sums need no rescaling.
+template <class T, class M, int DP, int WR>
+__global__ __launch_bounds__(64 * NW, (FWD_OCC<M, DP>)) void xattn_fwd_kernel(XArgs a) {
   typedef typename M::elem E;
-  constexpr int LD = DP + M::PAD, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
-  __shared__ __align__(16) E ks[KT * LD];
-  __shared__ __align__(16) E vs[KT * LD];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int tile = blockIdx.x % a.tiles;
-  const int64_t rest = blockIdx.x / a.tiles;
-  const int split = (int)(rest % a.splits);
-  const int64_t bh = rest / a.splits;
-  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
-  const int row = (tile * NW + wave) * 32 + (lane & 31);
+  constexpr int KT = FWD_KT<M, WR>, WK = NW / WR, NU = KT / 32 / WK;
+  constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  constexpr int TILE_BYTES = 2 * KT * DP * (int)sizeof(E);
+  constexpr int JOIN_BYTES = (NW - WR) * (DP * 32 + 128) * 4;
+  __shared__ __align__(16) char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
+  __shared__ uint32_t words[SPAN / 32];
+  E* ks = reinterpret_cast<E*>(lds);
+  E* vs = ks + KT * DP;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
+  const Job j = job_of(a);
+  const int row = (j.tile * WR + wr) * 32 + (lane & 31);
   const bool in = row < a.R;
-  const RowAt ra = row_at(a, hk, in ? row : 0);
-  const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
-  const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
-  const uint8_t* keep = a.keep ? a.keep + b * a.keep_bs : nullptr;
+  const RowAt ra = row_at(a, j.hk, in ? row : 0);
+  const T* k = static_cast<const T*>(a.k) + j.b * a.k_bs + j.hk * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + j.b * a.v_bs + j.hk * a.v_hs;
+  const uint8_t* keep = a.keep ? a.keep + j.b * a.keep_bs : nullptr;
+  const auto k_at = [&](int64_t r) { return k + r * a.k_ls; };
+  const auto v_at = [&](int64_t r) { return v + r * a.v_ls; };
   typename M::frag q[NC];
-  load_rows<T, M, DP>(q, static_cast<const T*>(a.q) + b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs,
+  load_rows<T, M, DP>(q, static_cast<const T*>(a.q) + j.b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs,
                       in, a.D, lane);
   f32x16 acc[DP / 32] = {};
-  float m = -INFINITY, l = 0.f;
-  const int k_lo = split * a.per_split, k_hi = min(a.Lk, k_lo + a.per_split);
-  for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
-    uint32_t bits[KT / 32];
-    uint32_t any = 0;
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u) any |= bits[u] = keep_bits(keep, k0 + 32 * u, k_hi, lane);
-    if (any == 0) continue;  // the same for every wave of the block
+  float m = -INFINITY, l = 0.f;  // of the unscaled scores
+  const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
+  Stage<T, M, DP, KT, 64 * NW> sk, sv;
+  for (int64_t base = k_lo; base < k_hi; base += SPAN) {
     __syncthreads();
-    stage<T, M, DP>(ks, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return k + r * a.k_ls; }, t,
-                    64 * NW);
-    stage<T, M, DP>(vs, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return v + r * a.v_ls; }, t,
-                    64 * NW);
+    span_words(words, keep, base, k_hi, t, 64 * NW);
     __syncthreads();
-    f32x16 s[KT / 32];
-    float top = m;
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u) {
-      s[u] = f32x16{};
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-        s[u] = M::mma(M::row(ks, LD, 32 * u, c * M::CHUNK, lane), q[c], s[u]);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = (bits[u] >> acc_row(r, lane)) & 1 ? s[u][r] * a.c : -INFINITY;
-        top = fmaxf(top, s[u][r]);
-      }
+    const int last = (int)min((int64_t)SPAN, k_hi - base);
+    int next = next_tile<KT>(words, 0, last);
+    if (next < last) {
+      sk.load(base + next, k_hi, a.D, k_at, t);
+      sv.load(base + next, k_hi, a.D, v_at, t);
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float base = top == -INFINITY ? 0.f : top;
-    const float alpha = exp2_fast(m - base);
-    m = top;
-    float sum = 0.f;
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = exp2_fast(s[u][r] - base);
-        sum += s[u][r];
+    while (next < last) {
+      const int cur = next;
+      __syncthreads();
+      sk.put(ks, nullptr, t);
+      sv.put(vs, words + cur / 32, t);
+      __syncthreads();
+      next = next_tile<KT>(words, cur + KT, last);
+      if (next < last) {
+        sk.load(base + next, k_hi, a.D, k_at, t);
+        sv.load(base + next, k_hi, a.D, v_at, t);
       }
-    l = l * alpha + sum;
+      const int u0 = wk * NU;
+      uint32_t bits[NU], any = 0, all = ~0u;
 #pragma unroll
-    for (int d = 0; d < DP / 32; ++d) acc[d] *= alpha;
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u)
-#pragma unroll
-      for (int c = 0; c < PC; ++c) {
-        const typename M::frag p = M::pack(s[u], c);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-          acc[d] = M::mma(M::col(vs, LD, 32 * u + c * M::CHUNK, 32 * d, lane), p, acc[d]);
+      for (int u = 0; u < NU; ++u) {
+        bits[u] = __builtin_amdgcn_readfirstlane(words[cur / 32 + u0 + u]);
+        any |= bits[u];
+        all &= bits[u];
       }
+      if (any == 0) continue;  // this wave's keys (its barriers come with the next tile)
+      f32x16 s[NU];
+      float top = m;
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        s[u] = f32x16{};
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+          s[u] = M::mma(row_frag<M, DP>(ks, 32 * (u0 + u), c, lane), q[c], s[u]);
+      }
+      if (all != ~0u) {
+#pragma unroll
+        for (int u = 0; u < NU; ++u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[u][r] = (bits[u] >> acc_row(r, lane)) & 1 ? s[u][r] : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+      top = halves(top, [](float x, float y) { return fmaxf(x, y); });
+      if (__ballot(top > m + a.slack)) {
+        const float alpha = top == -INFINITY ? 1.f : exp2_fast((m - top) * a.c);
+        m = top;
+        l *= alpha;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] *= alpha;
+      }
+      const float zero = m == -INFINITY ? 0.f : -m * a.c;
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[u][r] = exp2_fast(fmaf(s[u][r], a.c, zero));
+          sum[r & 1] += s[u][r];
+        }
+      l += sum[0] + sum[1];
+#pragma unroll
+      for (int u = 0; u < NU; ++u)
+#pragma unroll
+        for (int c = 0; c < PC; ++c) {
+          const typename M::frag p = M::pack(s[u], c);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+            acc[d] = M::mma(M::template col<DP>(vs, 32 * (u0 + u) + c * M::CHUNK, 32 * d, lane), p,
+                            acc[d]);
+        }
+    }
   }
-  l += __shfl_xor(l, 32, 64);
+  l = halves(l, [](float x, float y) { return x + y; });
+  if constexpr (WK > 1) {  // the waves along the keys
+    __syncthreads();
+    float* join = reinterpret_cast<float*>(lds);
+    constexpr int SLOT = DP * 32 + 128;
+    if (wk) {
+      float* o = join + ((wk - 1) * WR + wr) * SLOT;
+      acc_out(o, acc, lane);
+      o[DP * 32 + lane] = m;
+      o[DP * 32 + 64 + lane] = l;
+    }
+    __syncthreads();
+    if (wk) return;
+    for (int w = 0; w < WK - 1; ++w) {
+      const float* o = join + (w * WR + wr) * SLOT;
+      const float m2 = o[DP * 32 + lane], l2 = o[DP * 32 + 64 + lane], top = fmaxf(m, m2);
+      const float x = top == -INFINITY ? 1.f : exp2_fast((m - top) * a.c);
+      const float y = top == -INFINITY ? 1.f : exp2_fast((m2 - top) * a.c);
+      acc_join(o, acc, x, y, lane);
+      l = l * x + l2 * y;
+      m = top;
+    }
+  }
   if (!in) return;
   if (a.splits > 1) {
-    const int64_t at = ((int64_t)split * a.B * a.Hkv + bh) * a.R + row;
+    const int64_t at = ((int64_t)j.split * a.B * a.Hkv + j.bh) * a.R + row;
     float* o = a.part + at * a.D;
     for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
       if (d < a.D) store_f<float, 4>(o + d, x);
     });
     if (lane < 32) {
-      a.part_ms[2 * at] = m;
+      a.part_ms[2 * at] = m * a.c;
       a.part_ms[2 * at + 1] = l;
     }
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* o = static_cast<T*>(a.out) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+  T* o = static_cast<T*>(a.out) + (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) * a.D;
   for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
     const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
     if (d < a.D) store_f<T, 4>(o + d, y);
   });
   if (lane < 32 && a.lse)
-    a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m + log2f(l);
+    a.lse[((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m * a.c + log2f(l);
 }
 
 // The splits of a row: rescaled to their common maximum and summed in order.  A wave per row.
@@ -476,161 +644,240 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
   if (in && c == 0) a.delta[((int64_t)b * a.H + h) * a.Lq + i] = s;
 }
 
-// dQ: a wave per 32 rows, over the keys.
-template <class T, class M, int DP, int NW, int KT>
-__global__ __launch_bounds__(64 * NW) void xattn_dq_kernel(XArgs a) {
+// dQ: WR of the block's waves along the rows (32 each), the others along the staged keys.
+template <class M, int WR>
+constexpr int DQ_KT = sizeof(typename M::elem) == 2 ? (WR == 4 ? 64 : 128) : 32 * (NW / WR);
+
+template <class T, class M, int DP, int WR>
+__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP>)) void xattn_dq_kernel(XArgs a) {
   typedef typename M::elem E;
-  constexpr int LD = DP + M::PAD, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
-  __shared__ __align__(16) E ks[KT * LD];
-  __shared__ __align__(16) E vs[KT * LD];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int tile = blockIdx.x % a.tiles;
-  const int64_t rest = blockIdx.x / a.tiles;
-  const int split = (int)(rest % a.splits);
-  const int64_t bh = rest / a.splits;
-  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
-  const int row = (tile * NW + wave) * 32 + (lane & 31);
+  constexpr int KT = DQ_KT<M, WR>, WK = NW / WR, NU = KT / 32 / WK;
+  constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  constexpr int TILE_BYTES = 2 * KT * DP * (int)sizeof(E);
+  constexpr int JOIN_BYTES = (NW - WR) * DP * 32 * 4;
+  __shared__ __align__(16) char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
+  __shared__ uint32_t words[SPAN / 32];
+  E* ks = reinterpret_cast<E*>(lds);
+  E* vs = ks + KT * DP;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
+  const Job j = job_of(a);
+  const int row = (j.tile * WR + wr) * 32 + (lane & 31);
   const bool in = row < a.R;
-  const RowAt ra = row_at(a, hk, in ? row : 0);
-  const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
-  const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
-  const uint8_t* keep = a.keep ? a.keep + b * a.keep_bs : nullptr;
+  const RowAt ra = row_at(a, j.hk, in ? row : 0);
+  const T* k = static_cast<const T*>(a.k) + j.b * a.k_bs + j.hk * a.k_hs;
+  const T* v = static_cast<const T*>(a.v) + j.b * a.v_bs + j.hk * a.v_hs;
+  const uint8_t* keep = a.keep ? a.keep + j.b * a.keep_bs : nullptr;
+  const auto k_at = [&](int64_t r) { return k + r * a.k_ls; };
+  const auto v_at = [&](int64_t r) { return v + r * a.v_ls; };
   typename M::frag q[NC], go[NC];
-  load_rows<T, M, DP>(q, static_cast<const T*>(a.q) + b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs,
+  load_rows<T, M, DP>(q, static_cast<const T*>(a.q) + j.b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs,
                       in, a.D, lane);
   load_rows<T, M, DP>(go,
-                      static_cast<const T*>(a.dout) + b * a.do_bs + ra.i * a.do_ls +
+                      static_cast<const T*>(a.dout) + j.b * a.do_bs + ra.i * a.do_ls +
                           ra.h * a.do_hs,
                       in, a.D, lane);
-  const int64_t stat = ((int64_t)b * a.H + ra.h) * a.Lq + ra.i;
+  const int64_t stat = ((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i;
   const float lse = in ? a.lse[stat] : -INFINITY, delta = in ? a.delta[stat] : 0.f;
-  const bool some = lse != -INFINITY;
+  // a row without a key (and one that does not exist) has exponents of -inf: P = 0
+  const float neg = lse == -INFINITY ? -INFINITY : -lse;
   f32x16 acc[DP / 32] = {};
-  const int k_lo = split * a.per_split, k_hi = min(a.Lk, k_lo + a.per_split);
-  for (int k0 = k_lo; k0 < k_hi; k0 += KT) {
-    uint32_t bits[KT / 32];
-    uint32_t any = 0;
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u) any |= bits[u] = keep_bits(keep, k0 + 32 * u, k_hi, lane);
-    if (any == 0) continue;
+  const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
+  Stage<T, M, DP, KT, 64 * NW> sk, sv;
+  for (int64_t base = k_lo; base < k_hi; base += SPAN) {
     __syncthreads();
-    stage<T, M, DP>(ks, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return k + r * a.k_ls; }, t,
-                    64 * NW);
-    stage<T, M, DP>(vs, KT, k0, k_hi, a.D, keep, [&](int64_t r) { return v + r * a.v_ls; }, t,
-                    64 * NW);
+    span_words(words, keep, base, k_hi, t, 64 * NW);
     __syncthreads();
-#pragma unroll
-    for (int u = 0; u < KT / 32; ++u) {
-      f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        s = M::mma(M::row(ks, LD, 32 * u, c * M::CHUNK, lane), q[c], s);
-        dp = M::mma(M::row(vs, LD, 32 * u, c * M::CHUNK, lane), go[c], dp);
+    const int last = (int)min((int64_t)SPAN, k_hi - base);
+    int next = next_tile<KT>(words, 0, last);
+    if (next < last) {
+      sk.load(base + next, k_hi, a.D, k_at, t);
+      sv.load(base + next, k_hi, a.D, v_at, t);
+    }
+    while (next < last) {
+      const int cur = next;
+      __syncthreads();
+      sk.put(ks, words + cur / 32, t);
+      sv.put(vs, words + cur / 32, t);
+      __syncthreads();
+      next = next_tile<KT>(words, cur + KT, last);
+      if (next < last) {
+        sk.load(base + next, k_hi, a.D, k_at, t);
+        sv.load(base + next, k_hi, a.D, v_at, t);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const bool ok = ((bits[u] >> acc_row(r, lane)) & 1) && some;
-        s[r] = ok ? exp2_fast(fmaf(s[r], a.c, -lse)) * (dp[r] - delta) : 0.f;
-      }
+      for (int u = wk * NU; u < (wk + 1) * NU; ++u) {
+        const uint32_t bits = __builtin_amdgcn_readfirstlane(words[cur / 32 + u]);
+        if (bits == 0) continue;
+        f32x16 s = {}, dp = {};
 #pragma unroll
-      for (int c = 0; c < PC; ++c) {
-        const typename M::frag ds = M::pack(s, c);
+        for (int c = 0; c < NC; ++c) {
+          s = M::mma(row_frag<M, DP>(ks, 32 * u, c, lane), q[c], s);
+          dp = M::mma(row_frag<M, DP>(vs, 32 * u, c, lane), go[c], dp);
+        }
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-          acc[d] = M::mma(M::col(ks, LD, 32 * u + c * M::CHUNK, 32 * d, lane), ds, acc[d]);
+        for (int r = 0; r < 16; ++r)
+          s[r] = exp2_fast(fmaf(s[r], a.c, neg)) * (dp[r] - delta);
+        if (bits != ~0u)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = (bits >> acc_row(r, lane)) & 1 ? s[r] : 0.f;
+#pragma unroll
+        for (int c = 0; c < PC; ++c) {
+          const typename M::frag ds = M::pack(s, c);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d)
+            acc[d] = M::mma(M::template col<DP>(ks, 32 * u + c * M::CHUNK, 32 * d, lane), ds,
+                            acc[d]);
+        }
       }
     }
   }
+  if constexpr (WK > 1) {
+    __syncthreads();
+    float* join = reinterpret_cast<float*>(lds);
+    if (wk) acc_out(join + ((wk - 1) * WR + wr) * DP * 32, acc, lane);
+    __syncthreads();
+    if (wk) return;
+    for (int w = 0; w < WK - 1; ++w)
+      acc_join(join + (w * WR + wr) * DP * 32, acc, 1.f, 1.f, lane);
+  }
   if (!in) return;
   if (a.splits > 1) {
-    float* o = a.part + (((int64_t)split * a.B * a.Hkv + bh) * a.R + row) * a.D;
+    float* o = a.part + (((int64_t)j.split * a.B * a.Hkv + j.bh) * a.R + row) * a.D;
     for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
       if (d < a.D) store_f<float, 4>(o + d, x);
     });
     return;
   }
-  T* o = static_cast<T*>(a.dq) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+  T* o = static_cast<T*>(a.dq) + (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) * a.D;
   for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
     const float y[4] = {x[0] * a.scale, x[1] * a.scale, x[2] * a.scale, x[3] * a.scale};
     if (d < a.D) store_f<T, 4>(o + d, y);
   });
 }
 
-// dK, dV: a wave per 32 keys, over the rows of every head that shares them.
-template <class T, class M, int DP, int NW, int RT>
-__global__ __launch_bounds__(64 * NW) void xattn_dkv_kernel(XArgs a) {
+// dK, dV: WC of the block's waves along the keys (32 each), the others along the staged rows, over
+// the rows of every head that shares the keys.
+template <class M, int WC>
+constexpr int DKV_RT = sizeof(typename M::elem) == 2 && WC == NW ? 64 : 32 * (NW / WC);
+
+template <class T, class M, int DP, int WC>
+__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP>)) void xattn_dkv_kernel(XArgs a) {
   typedef typename M::elem E;
-  constexpr int LD = DP + M::PAD, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
-  __shared__ __align__(16) E qs[RT * LD];
-  __shared__ __align__(16) E gs[RT * LD];
-  __shared__ __align__(16) float st[2][RT];  // lse, delta
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int tile = blockIdx.x % a.tiles;
-  const int64_t rest = blockIdx.x / a.tiles;
-  const int split = (int)(rest % a.splits);
-  const int64_t bh = rest / a.splits;
-  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
-  const int key = (tile * NW + wave) * 32 + (lane & 31);
+  constexpr int RT = DKV_RT<M, WC>, WS = NW / WC, NU = RT / 32 / WS;
+  constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  constexpr int TILE_BYTES = 2 * RT * DP * (int)sizeof(E);
+  constexpr int JOIN_BYTES = (NW - WC) * DP * 32 * 4;  // dK, then dV
+  __shared__ __align__(16) char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
+  __shared__ __align__(16) float st[2][RT];  // -lse (-inf: a row without a key), delta
+  E* qs = reinterpret_cast<E*>(lds);
+  E* gs = qs + RT * DP;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wc = wave % WC, ws = wave / WC;
+  const Job j = job_of(a);
+  const int64_t key = ((int64_t)j.tile * WC + wc) * 32 + (lane & 31);
   const bool in = key < a.Lk;
-  const bool ok = in && (!a.keep || a.keep[b * a.keep_bs + key]);
+  const bool ok = in && (!a.keep || a.keep[j.b * a.keep_bs + key]);
   typename M::frag k[NC], v[NC];
-  load_rows<T, M, DP>(k, static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs + key * a.k_ls, ok,
-                      a.D, lane);
-  load_rows<T, M, DP>(v, static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs + key * a.v_ls, ok,
-                      a.D, lane);
-  const T* q = static_cast<const T*>(a.q) + b * a.q_bs;
-  const T* go = static_cast<const T*>(a.dout) + b * a.do_bs;
+  load_rows<T, M, DP>(k, static_cast<const T*>(a.k) + j.b * a.k_bs + j.hk * a.k_hs + key * a.k_ls,
+                      ok, a.D, lane);
+  load_rows<T, M, DP>(v, static_cast<const T*>(a.v) + j.b * a.v_bs + j.hk * a.v_hs + key * a.v_ls,
+                      ok, a.D, lane);
+  const T* q = static_cast<const T*>(a.q) + j.b * a.q_bs;
+  const T* go = static_cast<const T*>(a.dout) + j.b * a.do_bs;
+  const auto q_at = [&](int64_t r) {
+    const RowAt ra = row_at(a, j.hk, (int)r);
+    return q + ra.i * a.q_ls + ra.h * a.q_hs;
+  };
+  const auto g_at = [&](int64_t r) {
+    const RowAt ra = row_at(a, j.hk, (int)r);
+    return go + ra.i * a.do_ls + ra.h * a.do_hs;
+  };
   f32x16 dk[DP / 32] = {}, dv[DP / 32] = {};
-  const int r_lo = split * a.per_split, r_hi = min(a.R, r_lo + a.per_split);
+  const int r_lo = j.split * a.per_split, r_hi = min(a.R, r_lo + a.per_split);
   const bool live = __syncthreads_or(ok);  // a tile of padding has no gradient
+  const bool mine = __ballot(ok) != 0;
+  const bool whole = __ballot(ok) == ~0ull;
+  Stage<T, M, DP, RT, 64 * NW> sq, sg;
+  float stat[2] = {-INFINITY, 0.f};
+  const auto load = [&](int r0) {
+    sq.load(r0, r_hi, a.D, q_at, t);
+    sg.load(r0, r_hi, a.D, g_at, t);
+    if (t < RT) {
+      const bool there = r0 + t < r_hi;
+      const RowAt ra = row_at(a, j.hk, there ? r0 + t : 0);
+      const int64_t at = ((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i;
+      const float lse = there ? a.lse[at] : -INFINITY;
+      stat[0] = lse == -INFINITY ? -INFINITY : -lse;
+      stat[1] = there ? a.delta[at] : 0.f;
+    }
+  };
+  if (live && r_lo < r_hi) load(r_lo);
   for (int r0 = r_lo; live && r0 < r_hi; r0 += RT) {
     __syncthreads();
-    stage<T, M, DP>(qs, RT, r0, r_hi, a.D, nullptr, [&](int64_t r) {
-      const RowAt ra = row_at(a, hk, (int)r);
-      return q + ra.i * a.q_ls + ra.h * a.q_hs;
-    }, t, 64 * NW);
-    stage<T, M, DP>(gs, RT, r0, r_hi, a.D, nullptr, [&](int64_t r) {
-      const RowAt ra = row_at(a, hk, (int)r);
-      return go + ra.i * a.do_ls + ra.h * a.do_hs;
-    }, t, 64 * NW);
-    for (int i = t; i < RT; i += 64 * NW) {
-      const bool there = r0 + i < r_hi;
-      const RowAt ra = row_at(a, hk, there ? r0 + i : 0);
-      const int64_t at = ((int64_t)b * a.H + ra.h) * a.Lq + ra.i;
-      st[0][i] = there ? a.lse[at] : -INFINITY;
-      st[1][i] = there ? a.delta[at] : 0.f;
+    sq.put(qs, nullptr, t);
+    sg.put(gs, nullptr, t);
+    if (t < RT) {
+      st[0][t] = stat[0];
+      st[1][t] = stat[1];
     }
     __syncthreads();
+    if (r0 + RT < r_hi) load(r0 + RT);
+    if (!mine) continue;
 #pragma unroll
-    for (int u = 0; u < RT / 32; ++u) {
+    for (int u = ws * NU; u < (ws + 1) * NU; ++u) {
       f32x16 s = {}, dp = {};
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        s = M::mma(M::row(qs, LD, 32 * u, c * M::CHUNK, lane), k[c], s);
-        dp = M::mma(M::row(gs, LD, 32 * u, c * M::CHUNK, lane), v[c], dp);
+        s = M::mma(row_frag<M, DP>(qs, 32 * u, c, lane), k[c], s);
+        dp = M::mma(row_frag<M, DP>(gs, 32 * u, c, lane), v[c], dp);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = 32 * u + acc_row(r, lane);
-        const float lse = st[0][i];
-        const bool p = ok && lse != -INFINITY;
-        s[r] = p ? exp2_fast(fmaf(s[r], a.c, -lse)) : 0.f;
-        dp[r] = p ? s[r] * (dp[r] - st[1][i]) : 0.f;
+      for (int r4 = 0; r4 < 4; ++r4) {
+        const int i = 32 * u + acc_row(4 * r4, lane);
+        const f32x4 neg = *reinterpret_cast<const f32x4*>(&st[0][i]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&st[1][i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = 4 * r4 + e;
+          s[r] = exp2_fast(fmaf(s[r], a.c, neg[e]));
+          dp[r] = s[r] * (dp[r] - delta[e]);
+        }
       }
+      if (!whole)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = ok ? s[r] : 0.f;
+          dp[r] = ok ? dp[r] : 0.f;
+        }
 #pragma unroll
       for (int c = 0; c < PC; ++c) {
         const typename M::frag p = M::pack(s, c), ds = M::pack(dp, c);
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = M::mma(M::col(gs, LD, 32 * u + c * M::CHUNK, 32 * d, lane), p, dv[d]);
-          dk[d] = M::mma(M::col(qs, LD, 32 * u + c * M::CHUNK, 32 * d, lane), ds, dk[d]);
+          dv[d] = M::mma(M::template col<DP>(gs, 32 * u + c * M::CHUNK, 32 * d, lane), p, dv[d]);
+          dk[d] = M::mma(M::template col<DP>(qs, 32 * u + c * M::CHUNK, 32 * d, lane), ds, dk[d]);
         }
       }
     }
   }
+  if constexpr (WS > 1) {
+    float* join = reinterpret_cast<float*>(lds);
+    const auto join_waves = [&](f32x16 (&x)[DP / 32]) {
+      __syncthreads();
+      if (ws) acc_out(join + ((ws - 1) * WC + wc) * DP * 32, x, lane);
+      __syncthreads();
+      if (!ws)
+        for (int w = 0; w < WS - 1; ++w)
+          acc_join(join + (w * WC + wc) * DP * 32, x, 1.f, 1.f, lane);
+    };
+    join_waves(dk);
+    join_waves(dv);
+    if (ws) return;
+  }
   if (!in) return;
   if (a.splits > 1) {
-    const int64_t at = (((int64_t)split * a.B * a.Hkv + bh) * a.Lk + key) * a.D;
+    const int64_t at = (((int64_t)j.split * a.B * a.Hkv + j.bh) * a.Lk + key) * a.D;
     for_runs<DP>(dk, lane, [&](int d, const float (&x)[4]) {
       if (d < a.D) store_f<float, 4>(a.part + at + d, x);
     });
@@ -639,7 +886,7 @@ __global__ __launch_bounds__(64 * NW) void xattn_dkv_kernel(XArgs a) {
     });
     return;
   }
-  const int64_t at = (((int64_t)b * a.Lk + key) * a.Hkv + hk) * a.D;
+  const int64_t at = (((int64_t)j.b * a.Lk + key) * a.Hkv + j.hk) * a.D;
   for_runs<DP>(dk, lane, [&](int d, const float (&x)[4]) {
     const float y[4] = {x[0] * a.scale, x[1] * a.scale, x[2] * a.scale, x[3] * a.scale};
     if (d < a.D) store_f<T, 4>(static_cast<T*>(a.dk) + at + d, y);
@@ -695,7 +942,7 @@ struct Tiling {
 };
 Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t least, int unit) {
   Tiling t;
-  t.nw = n <= 32 ? 1 : n <= 64 ? 2 : 4;
+  t.nw = n <= 32 ? 1 : n <= 64 ? 2 : NW;
   t.tiles = (int)std::max<int64_t>(1, cdiv(n, 32 * t.nw));
   int64_t s = cdiv(want, std::max<int64_t>(1, heads * t.tiles));
   s = std::max<int64_t>(1, std::min(s, other / least));
@@ -721,10 +968,10 @@ XPlan xattn_plan(const int64_t* dims) {
     p.fwd = tiling(heads, 1, Lk, 1024, 256, 64);
     p.fwd.tiles = 1;
   } else {
-    p.fwd = tiling(heads, R, Lk, 512, 128, 64);
+    p.fwd = tiling(heads, R, Lk, 256, 256, 128);
   }
-  p.dq = tiling(heads, R, Lk, 512, 128, 64);
-  p.dkv = tiling(heads, Lk, R, 512, 128, 64);
+  p.dq = tiling(heads, R, Lk, 256, 256, 128);
+  p.dkv = tiling(heads, Lk, R, 256, 256, 128);
   int64_t at = 0;
   if (p.fwd.splits > 1) at = up256(p.fwd.splits * heads * R * D * 4);
   p.part_ms = at;
@@ -768,8 +1015,13 @@ XArgs xattn_args(const void* q, const void* k, const void* v, const uint8_t* kee
   a.Lq = (int)dims[3]; a.Lk = (int)dims[4]; a.D = (int)dims[5];
   a.G = a.H / a.Hkv;
   a.R = a.G * a.Lq;
+  // with s = 30 + ceil(log2 Lq), ceil(2^s / Lq) Lq passes 2^s by less than Lq: exact below 2^30
+  a.lq_shift = 30;
+  while (((int64_t)1 << (a.lq_shift - 30)) < a.Lq) ++a.lq_shift;
+  a.lq_mul = (uint64_t)cdiv((int64_t)1 << a.lq_shift, std::max(a.Lq, 1));
   a.scale = scale;
-  a.c = scale * LOG2E;
+  a.c = std::max(scale * LOG2E, 1e-30f);  // scale 0: exponents of 0, whatever the scores
+  a.slack = 8.f / a.c;
   return a;
 }
 
@@ -814,15 +1066,14 @@ int few_rows(const XArgs& a, unsigned blocks, hipStream_t s) {
 template <class T>
 int xattn_forward(XArgs a, const XPlan& p, hipStream_t s) {
   typedef typename MmaOf<T>::type M;
-  constexpr int KT = sizeof(typename M::elem) == 2 ? 64 : 32;
   const unsigned blocks = xattn_tile(a, p.fwd);
   if (p.few) {
     MPR_TRY(a.R == 1 ? (few_rows<T, 1>(a, blocks, s)) : a.R == 2 ? (few_rows<T, 2>(a, blocks, s))
             : a.R <= 4 ? (few_rows<T, 4>(a, blocks, s)) : (few_rows<T, 8>(a, blocks, s)));
   } else {
     MPR_TRY(by_tile(a.D, p.fwd.nw, [&](auto dp, auto nw) -> int {
-      constexpr int DP = dp, NW = nw;
-      xattn_fwd_kernel<T, M, DP, NW, NW == 4 ? KT : 32><<<blocks, 64 * NW, 0, s>>>(a);
+      constexpr int DP = dp, WR = nw;
+      xattn_fwd_kernel<T, M, DP, WR><<<blocks, 64 * NW, 0, s>>>(a);
       MPR_LAUNCHED();
       return MPR_OK;
     }));
@@ -838,7 +1089,6 @@ int xattn_forward(XArgs a, const XPlan& p, hipStream_t s) {
 template <class T>
 int xattn_backward(XArgs a, const XPlan& p, hipStream_t s) {
   typedef typename MmaOf<T>::type M;
-  constexpr int KT = sizeof(typename M::elem) == 2 ? 64 : 32;
   const int64_t rows = (int64_t)a.B * a.Lq * a.H, heads = (int64_t)a.B * a.Hkv;
   if (rows) {
     xattn_delta_kernel<T><<<dim3((unsigned)cdiv(rows, 16)), 256, 0, s>>>(a);
@@ -847,8 +1097,8 @@ int xattn_backward(XArgs a, const XPlan& p, hipStream_t s) {
   if (a.Lk && a.dk) {
     const unsigned blocks = xattn_tile(a, p.dkv);
     MPR_TRY(by_tile(a.D, p.dkv.nw, [&](auto dp, auto nw) -> int {
-      constexpr int DP = dp, NW = nw;
-      xattn_dkv_kernel<T, M, DP, NW, 32><<<blocks, 64 * NW, 0, s>>>(a);
+      constexpr int DP = dp, WC = nw;
+      xattn_dkv_kernel<T, M, DP, WC><<<blocks, 64 * NW, 0, s>>>(a);
       MPR_LAUNCHED();
       return MPR_OK;
     }));
@@ -860,8 +1110,8 @@ int xattn_backward(XArgs a, const XPlan& p, hipStream_t s) {
   if (rows && a.dq) {
     const unsigned blocks = xattn_tile(a, p.dq);
     MPR_TRY(by_tile(a.D, p.dq.nw, [&](auto dp, auto nw) -> int {
-      constexpr int DP = dp, NW = nw;
-      xattn_dq_kernel<T, M, DP, NW, NW == 4 ? KT : 32><<<blocks, 64 * NW, 0, s>>>(a);
+      constexpr int DP = dp, WR = nw;
+      xattn_dq_kernel<T, M, DP, WR><<<blocks, 64 * NW, 0, s>>>(a);
       MPR_LAUNCHED();
       return MPR_OK;
     }));
@@ -897,7 +1147,7 @@ int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* ke
                   void* ws, int64_t ws_bytes, void* stream) {
   return ops_call("xattn_fwd", [&]() -> int {
     MPR_TRY(xattn_check("xattn_fwd", dims, dtype));
-    MPR_REQUIRE(strides, "xattn_fwd: no strides");
+    MPR_REQUIRE(strides && scale >= 0.f, "xattn_fwd: no strides, or a scale below 0");
     if (dims[0] * dims[3] == 0) return MPR_OK;
     MPR_REQUIRE(q && out && (dims[4] == 0 || (k && v)), "xattn_fwd: null pointer");
     const XPlan p = xattn_plan(dims);
@@ -921,7 +1171,7 @@ int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* ke
                   int64_t ws_bytes, void* stream) {
   return ops_call("xattn_bwd", [&]() -> int {
     MPR_TRY(xattn_check("xattn_bwd", dims, dtype));
-    MPR_REQUIRE(strides, "xattn_bwd: no strides");
+    MPR_REQUIRE(strides && scale >= 0.f, "xattn_bwd: no strides, or a scale below 0");
     if (dims[0] * (dims[3] + dims[4]) == 0) return MPR_OK;
     MPR_REQUIRE(dims[3] == 0 || (q && out && lse && dout), "xattn_bwd: null pointer");
     MPR_REQUIRE(dims[4] == 0 || (k && v), "xattn_bwd: null pointer");

@@ -272,6 +272,8 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
             raise ValueError(f"cross_attention: key_mask {tuple(key_mask.shape)}, "
                              f"needed [{B}, {Lk}]")
     _on_gpu(q, "cross_attention")
+    if scale < 0.0:  # the kernels' running maximum is of unscaled scores
+        q, scale = -q, -scale
     if key_mask is not None:
         keep = key_mask if key_mask.dtype == torch.bool else key_mask != 0
         keep = _rows(keep.detach().expand(B, Lk)).view(torch.uint8)
