@@ -8,6 +8,7 @@
 // windows' fp32 partial sums, in window order.
 //
 // An id outside [0, V) reads nothing: its output row is NaN, and it has no gradient.
+#include <algorithm>
 #include <cmath>
 
 #include "ops.h"
@@ -67,6 +68,7 @@ constexpr int SORT_WAVES = SORT_THREADS / 64;
 constexpr int SORT_ITEMS = 4;  // per thread
 constexpr int SORT_TILE = SORT_THREADS * SORT_ITEMS;
 constexpr int SORT_BLOCKS = 256;
+constexpr int SORT_ONE = 16 * SORT_THREADS;  // positions that one launch sorts
 constexpr int DIGITS = 256;
 
 struct SortPlan {
@@ -123,6 +125,130 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_count_kernel(KeySrc src, in
   if (t < DIGITS) hist[(int64_t)blockIdx.x * DIGITS + t] = cnt[t];
 }
 
+// The exclusive sums of the first 256 threads' values (every thread of the block calls it).
+__device__ __forceinline__ uint32_t scan_digits(uint32_t v, uint32_t* part) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  uint32_t s = v;
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t x = __shfl_up(s, off, 64);
+    if (lane >= off) s += x;
+  }
+  if (wave < 4 && lane == 63) part[wave] = s;
+  __syncthreads();
+  for (int w = 0; w < 4; ++w)
+    if (w < wave && wave < 4) s += part[w];
+  return s - v;
+}
+
+// The rank of an item among those of its digit that this wave has met, this round's lower lanes
+// included; cnt: the wave's counts.  Lanes run in lockstep: every lane reads the count before the
+// first lane of its digit raises it (the fences keep the compiler from moving the accesses).
+__device__ __forceinline__ uint32_t digit_rank(uint32_t* cnt, uint32_t dig, bool in, int bits,
+                                               int lane) {
+  uint64_t same = __ballot(in);  // the lanes that hold this digit
+  for (int b = 0; b < bits; ++b) {
+    const uint64_t m = __ballot((dig >> b) & 1);
+    same &= (dig >> b) & 1 ? m : ~m;
+  }
+  const uint32_t old = in ? *(volatile uint32_t*)&cnt[dig] : 0;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const uint64_t below = same & ((1ull << lane) - 1);
+  if (in && below == 0) *(volatile uint32_t*)&cnt[dig] = old + (uint32_t)__popcll(same);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  return old + (uint32_t)__popcll(below);
+}
+
+// Up to ITEMS * SORT_THREADS positions in one launch: block b sorts the tokens [b range, (b + 1)
+// range) by itself.  It reads every id, counts those below its range (which says where its part of
+// the result begins) and keeps its own in the order of their positions; one counting pass over
+// `range` digits then ranks them.  Reading 16384 ids in 128 blocks costs less than the launches
+// that sharing them would take: 8992 ids 9 us against 28 us for the two passes above.
+constexpr int RANGE_MAX = 1024;
+template <int ITEMS>
+__global__ __launch_bounds__(SORT_THREADS) void sort_range_kernel(KeySrc src, int n, uint32_t range,
+                                                                  int bits, uint32_t* key_out,
+                                                                  uint32_t* pos_out) {
+  __shared__ uint32_t item[ITEMS * SORT_THREADS];  // token - lo (16 bits), position (14 bits)
+  __shared__ uint32_t wcnt[SORT_WAVES][RANGE_MAX];
+  __shared__ uint32_t mine[SORT_WAVES], less[SORT_WAVES], part[SORT_WAVES];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const uint32_t lo = blockIdx.x * range, hi = min(lo + range, (uint32_t)src.V + 1);
+  uint32_t key[ITEMS], n_mine = 0, n_less = 0;
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    const int i = (wave * ITEMS + r) * 64 + lane;
+    key[r] = i < n ? key_at(src, i) : ~0u;
+  }
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    n_less += (uint32_t)__popcll(__ballot(key[r] < lo));
+    n_mine += (uint32_t)__popcll(__ballot(key[r] >= lo && key[r] < hi));
+  }
+  if (lane == 0) {
+    mine[wave] = n_mine;
+    less[wave] = n_less;
+  }
+  for (uint32_t d = lane; d < range; d += 64) wcnt[wave][d] = 0;
+  __syncthreads();
+  uint32_t base = 0, total = 0, at = 0;
+  for (int w = 0; w < SORT_WAVES; ++w) {
+    base += less[w];
+    if (w < wave) at += mine[w];
+    total += mine[w];
+  }
+  if (total == 0) return;
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    const bool in = key[r] >= lo && key[r] < hi;
+    const uint64_t m = __ballot(in);
+    if (in)
+      item[at + (uint32_t)__popcll(m & ((1ull << lane) - 1))] =
+          (key[r] - lo) << 16 | (uint32_t)((wave * ITEMS + r) * 64 + lane);
+    at += (uint32_t)__popcll(m);
+  }
+  __syncthreads();
+  const int rounds = (int)((total + SORT_THREADS - 1) / SORT_THREADS);
+  uint32_t mark[ITEMS];  // an item's place among those of its token
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    if (r >= rounds) break;
+    const uint32_t i = (uint32_t)((wave * rounds + r) * 64 + lane);
+    const bool in = i < total;
+    mark[r] = digit_rank(wcnt[wave], in ? item[i] >> 16 : 0, in, bits, lane);
+  }
+  __syncthreads();
+  uint32_t count = 0;  // of token lo + t
+  if (t < (int)range)
+    for (int w = 0; w < SORT_WAVES; ++w) count += wcnt[w][t];
+  uint32_t sum = count;
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t x = __shfl_up(sum, off, 64);
+    if (lane >= off) sum += x;
+  }
+  if (lane == 63) part[wave] = sum;
+  __syncthreads();
+  uint32_t first = base + sum - count;
+  for (int w = 0; w < wave; ++w) first += part[w];
+  if (t < (int)range)
+    for (int w = 0; w < SORT_WAVES; ++w) {
+      const uint32_t c = wcnt[w][t];
+      wcnt[w][t] = first;
+      first += c;
+    }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < ITEMS; ++r) {
+    if (r >= rounds) break;
+    const uint32_t i = (uint32_t)((wave * rounds + r) * 64 + lane);
+    if (i >= total) continue;
+    const uint32_t x = item[i], to = wcnt[wave][x >> 16] + mark[r];
+    key_out[to] = lo + (x >> 16);
+    pos_out[to] = x & 0xFFFF;
+  }
+}
+
 __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(KeySrc src, int64_t n,
                                                                  int64_t tiles_per_block,
                                                                  int shift, int bits,
@@ -130,28 +256,19 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(KeySrc src, int
                                                                  uint32_t* key_out,
                                                                  uint32_t* pos_out) {
   __shared__ uint32_t base[DIGITS];                // next place of each digit
-  __shared__ uint32_t scan[DIGITS];
+  __shared__ uint32_t part[4];
   __shared__ uint32_t wcnt[SORT_WAVES][DIGITS];    // per wave: items of the digit, then their base
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const uint32_t mask = (1u << bits) - 1;
   uint32_t before = 0, total = 0;
-  if (t < DIGITS) {
+  if (t < DIGITS)
     for (int b = 0; b < (int)gridDim.x; ++b) {
       const uint32_t h = hist[(int64_t)b * DIGITS + t];
       if (b < (int)blockIdx.x) before += h;
       total += h;
     }
-    scan[t] = total;
-  }
-  __syncthreads();
-  for (int off = 1; off < DIGITS; off <<= 1) {
-    uint32_t v = 0;
-    if (t < DIGITS && t >= off) v = scan[t - off];
-    __syncthreads();
-    if (t < DIGITS) scan[t] += v;
-    __syncthreads();
-  }
-  if (t < DIGITS) base[t] = scan[t] - total + before;
+  const uint32_t smaller = scan_digits(total, part);
+  if (t < DIGITS) base[t] = smaller + before;
   const int64_t lo = (int64_t)blockIdx.x * tiles_per_block * SORT_TILE;
   const int64_t hi = min(n, lo + tiles_per_block * SORT_TILE);
   for (int64_t tile = lo; tile < hi; tile += SORT_TILE) {
@@ -164,23 +281,7 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(KeySrc src, int
       const bool in = i < hi;
       key[r] = in ? key_at(src, i) : 0;
       pos[r] = in ? (src.pos ? src.pos[i] : (uint32_t)i) : 0;
-      const uint32_t dig = (key[r] >> shift) & mask;
-      uint64_t same = __ballot(in);  // the lanes that hold this digit
-      for (int b = 0; b < bits; ++b) {
-        const uint64_t m = __ballot((dig >> b) & 1);
-        same &= (dig >> b) & 1 ? m : ~m;
-      }
-      // a wave's lanes run in lockstep: every lane reads the count before the first lane of its
-      // digit raises it (the fences keep the compiler from moving the accesses)
-      const uint32_t old = in ? *(volatile uint32_t*)&wcnt[wave][dig] : 0;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      const uint64_t below = same & ((1ull << lane) - 1);
-      rank[r] = old + (uint32_t)__popcll(below);
-      if (in && below == 0)
-        *(volatile uint32_t*)&wcnt[wave][dig] = old + (uint32_t)__popcll(same);
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      rank[r] = digit_rank(wcnt[wave], (key[r] >> shift) & mask, in, bits, lane);
     }
     __syncthreads();
     if (t < DIGITS) {
@@ -485,7 +586,19 @@ int mpr_embed_grad(const void* dout, int32_t dtype, int64_t ld, const void* ids,
                           reinterpret_cast<uint32_t*>(w + p.pos[1])};
       uint32_t* hist = reinterpret_cast<uint32_t*>(w + p.hist);
       KeySrc src{ids, ids64, V, padding_idx, nullptr, nullptr};
-      for (int i = 0; i < p.sort.passes; ++i) {
+      const int64_t range = std::max<int64_t>(64, cdiv(V + 1, 128));
+      const bool one = n <= SORT_ONE && range <= RANGE_MAX;
+      if (one) {
+        int bits = 1;
+        while ((int64_t)1 << bits < range) ++bits;
+        const auto sort = n <= 4 * SORT_THREADS ? sort_range_kernel<4> : sort_range_kernel<16>;
+        sort<<<dim3((unsigned)cdiv(V + 1, range)), SORT_THREADS, 0, s>>>(
+            src, (int)n, (uint32_t)range, bits, key[0], pos[0]);
+        MPR_LAUNCHED();
+        src.key = key[0];
+        src.pos = pos[0];
+      }
+      for (int i = 0; !one && i < p.sort.passes; ++i) {
         const int shift = i * p.sort.bits;
         sort_count_kernel<<<p.sort.blocks, SORT_THREADS, 0, s>>>(src, n, p.sort.tiles_per_block,
                                                                  shift, p.sort.bits, hist);

@@ -152,18 +152,50 @@ __global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable tab,
   clip_scale_of(tab.types[i], tab.in[i], tab.out[i], at, n, coef, threadIdx.x, CLIP_THREADS);
 }
 
+// Few values: one block does it all, a wave per unit of ONE_UNIT of them (three launches cost more
+// than the reads).
+constexpr int ONE_UNIT = 1024, ONE_UNITS = 128;
+__global__ __launch_bounds__(1024) void clip_one_kernel(ClipTable tab, int units, int scale,
+                                                        double max_norm, double eps, float* norm) {
+  __shared__ double red[16];
+  __shared__ float coef;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double s = 0.0;
+  for (int u = wave; u < units; u += 16) {
+    const int i = clip_find(tab, u);
+    const int64_t at = (int64_t)(u - tab.chunk0[i]) * ONE_UNIT;
+    const int64_t n = min((int64_t)ONE_UNIT, tab.n[i] - at);
+    s += clip_sumsq_of(tab.types[i] & 15, tab.in[i], at, n, lane, 64);
+  }
+  s = block_sum<1024>(s, red);
+  if (threadIdx.x == 0) {
+    const double r = sqrt(s);
+    norm[0] = (float)r;
+    coef = clip_coef(r, max_norm, eps);
+  }
+  __syncthreads();
+  for (int u = wave; scale && u < units; u += 16) {
+    const int i = clip_find(tab, u);
+    if (coef == 1.f && tab.in[i] == tab.out[i]) continue;
+    const int64_t at = (int64_t)(u - tab.chunk0[i]) * ONE_UNIT;
+    const int64_t n = min((int64_t)ONE_UNIT, tab.n[i] - at);
+    clip_scale_of(tab.types[i], tab.in[i], tab.out[i], at, n, coef, lane, 64);
+  }
+}
+
 struct Span {
   uintptr_t a, b;
 };
 
 // The rest of the tensors' table from item `i` on, at most CLIP_TABLE tensors; returns the next.
-int clip_fill(ClipTable& tab, const int64_t* desc, int n, int i, int64_t* chunks) {
+int clip_fill(ClipTable& tab, const int64_t* desc, int n, int i, int64_t* chunks,
+              int chunk = CHUNK) {
   int64_t c = 0;
   tab.count = 0;
   for (; i < n && tab.count < CLIP_TABLE; ++i) {
     const int64_t* d = desc + 5 * (int64_t)i;
     if (d[1] == 0) continue;
-    const int64_t own = cdiv(d[1], CHUNK);
+    const int64_t own = cdiv(d[1], chunk);
     if (c + own > MAX_GRID_X) break;
     const int k = tab.count++;
     tab.in[k] = reinterpret_cast<const void*>(d[0]);
@@ -244,9 +276,17 @@ int mpr_clip_grads(int32_t n, const int64_t* desc, double max_norm, double eps, 
     double* partial = reinterpret_cast<double*>(st + 1);
     ClipTable tab;
     int64_t done = 0, c = 0;
+    if (chunks <= ONE_UNITS && clip_fill(tab, desc, n, 0, &c, ONE_UNIT) == n && c <= ONE_UNITS) {
+      clip_one_kernel<<<1, 1024, 0, s>>>(tab, (int)c, scale, max_norm, eps, norm);
+      MPR_LAUNCHED();
+      return MPR_OK;
+    }
+    std::vector<int> first;  // the tensor that each launch begins with
     for (int i = 0; i < n;) {
+      const int from = i;
       i = clip_fill(tab, desc, n, i, &c);
       if (c == 0) continue;
+      first.push_back(from);
       clip_norm_kernel<<<dim3((unsigned)c), CLIP_THREADS, 0, s>>>(tab, partial + done);
       MPR_LAUNCHED();
       done += c;
@@ -254,9 +294,8 @@ int mpr_clip_grads(int32_t n, const int64_t* desc, double max_norm, double eps, 
     clip_finish_kernel<<<1, 1024, 0, s>>>(partial, chunks, max_norm, eps, norm, st);
     MPR_LAUNCHED();
     if (!scale) return MPR_OK;  // the norm alone
-    for (int i = 0; i < n;) {
-      i = clip_fill(tab, desc, n, i, &c);
-      if (c == 0) continue;
+    for (size_t k = first.size(); k-- > 0;) {
+      clip_fill(tab, desc, n, first[k], &c);
       clip_scale_kernel<<<dim3((unsigned)c), CLIP_THREADS, 0, s>>>(tab, st);
       MPR_LAUNCHED();
     }

@@ -133,10 +133,10 @@ __global__ __launch_bounds__(256) void lp_sequence_kernel(const T* x, LpArgs a, 
   }
 }
 
-// The pairs of the batch (one block): loss, and dlp of every sequence for a loss gradient of 1.
-__global__ __launch_bounds__(1024) void lp_pairs_kernel(const double* lp, const float* ref,
-                                                        int64_t P, double beta, double eps,
-                                                        float* loss, float* dlp) {
+// The pairs of the batch by one block of 1024: loss, and dlp of every sequence for a loss gradient
+// of 1.
+__device__ __forceinline__ void lp_pairs(const double* lp, const float* ref, int64_t P, double beta,
+                                         double eps, float* loss, float* dlp) {
   __shared__ double red[16];
   double sum = 0.0;
   for (int64_t p = threadIdx.x; p < P; p += 1024) {
@@ -154,6 +154,32 @@ __global__ __launch_bounds__(1024) void lp_pairs_kernel(const double* lp, const 
     for (int w = 1; w < 16; ++w) sum += red[w];
     loss[0] = (float)(sum / (double)P);
   }
+}
+
+__global__ __launch_bounds__(1024) void lp_pairs_kernel(const double* lp, const float* ref,
+                                                        int64_t P, double beta, double eps,
+                                                        float* loss, float* dlp) {
+  lp_pairs(lp, ref, P, beta, eps, loss, dlp);
+}
+
+// Few sequences: both in one launch, a wave for each sequence in turn.
+constexpr int LP_FEW = 64;
+template <class T>
+__global__ __launch_bounds__(1024) void lp_few_kernel(const T* x, LpArgs a, const MaxSum* stat,
+                                                      MaxSum* row_stat, float* logps,
+                                                      const float* ref, double beta, double eps,
+                                                      float* loss, float* dlp) {
+  __shared__ double lp64[LP_FEW];
+  const int lane = threadIdx.x & 63;
+  for (int s = threadIdx.x >> 6; s < a.S; s += 16) {
+    const double lp = lp_sequence(x, a, stat, row_stat, s, lane);
+    if (lane == 0) {
+      logps[s] = (float)lp;
+      lp64[s] = lp;
+    }
+  }
+  __syncthreads();
+  lp_pairs(lp64, ref, a.S / 2, beta, eps, loss, dlp);
 }
 
 template <class T>
@@ -270,12 +296,18 @@ int mpr_logps_fwd(const void* logits, int32_t dtype, int64_t S, int64_t T, int64
         lp_stats_kernel<X><<<dim3((unsigned)p.rows, p.split), LP_THREADS, 0, s>>>(x, a, stat);
         MPR_LAUNCHED();
       }
+      if (loss && S <= LP_FEW) {
+        lp_few_kernel<X><<<1, 1024, 0, s>>>(x, a, stat, reinterpret_cast<MaxSum*>(row_stat), logps,
+                                            ref, beta, label_smoothing, loss, dlogps);
+        MPR_LAUNCHED();
+        return MPR_OK;
+      }
       lp_sequence_kernel<X><<<dim3((unsigned)cdiv(S, 4)), 256, 0, s>>>(
           x, a, stat, reinterpret_cast<MaxSum*>(row_stat), logps, lp64);
       MPR_LAUNCHED();
       return MPR_OK;
     }));
-    if (!loss) return MPR_OK;
+    if (!loss || S <= LP_FEW) return MPR_OK;
     lp_pairs_kernel<<<1, 1024, 0, s>>>(lp64, ref, S / 2, beta, label_smoothing, loss, dlogps);
     MPR_LAUNCHED();
     return MPR_OK;

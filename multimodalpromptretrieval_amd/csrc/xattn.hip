@@ -290,8 +290,8 @@ constexpr int NW = 4;  // waves of a block
 // Waves a SIMD is to hold (what the registers are shared by).
 template <class M, int DP>
 constexpr int FWD_OCC = sizeof(typename M::elem) == 2 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 2 : 1);
-template <class M, int DP>
-constexpr int BWD_OCC = sizeof(typename M::elem) == 2 && DP == 64 ? 2 : 1;
+template <class M, int DP, int W>
+constexpr int BWD_OCC = DP == 64 && (sizeof(typename M::elem) == 2 || W == NW) ? 2 : 1;
 // The block's waves: WR of them along the rows (32 each), NW / WR along the staged keys.
 // KT keys are staged at a time.
 template <class M, int WR>
@@ -491,20 +491,44 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 }
 
 // ---- a few rows (single tokens) ------------------------------------------------------------------
-// The keys and values are read once and that is all the time there is: no matrix core, no LDS until
-// the end.  LPR lanes read a key's row, 16 bytes each, so a wave reads 64 / LPR keys at a time; each
-// such group of lanes keeps its own running maximum, sum and output share of every row, and they
-// are joined when the keys are done.
-constexpr int FEW_WAVES = 4, FEW_AHEAD = 4;
+// The keys and values are read once and that is all the time there is: no matrix core, and LDS only
+// for the mask's bits and the end.  LPR lanes read a key's row, 16 bytes each, so a wave reads 64 /
+// LPR keys at a time; each such group of lanes keeps its own running maximum, sum and output share
+// of every row, and they are joined when the keys are done.  The wave's next FEW_AHEAD reads are on
+// their way while the present ones are computed.
+constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
+
+template <int CTRL>
+__device__ __forceinline__ float permuted(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+// the sum over neighbouring groups of LPR lanes, in all of them (no LDS: lane permutations)
+template <int LPR>
+__device__ __forceinline__ float group_add(float x) {
+  x += permuted<0xB1>(x);   // lane ^ 1
+  x += permuted<0x4E>(x);   // lane ^ 2
+  x += permuted<0x141>(x);  // mirrored in 8: the other four
+  if constexpr (LPR >= 16) x += permuted<0x140>(x);  // mirrored in 16: the other eight
+  if constexpr (LPR == 32) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  }
+  return x;
+}
+
 template <class T, int LPR, int NR>
 __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
-  constexpr int N = VEC16<T>, KPI = 64 / LPR;
+  constexpr int N = VEC16<T>, KPI = 64 / LPR, GROUP = KPI * FEW_AHEAD, STEP = FEW_WAVES * GROUP;
+  constexpr uint32_t GROUP_BITS = GROUP == 32 ? ~0u : (1u << (GROUP % 32)) - 1;
   __shared__ float so[FEW_WAVES][NR][LPR * N];
   __shared__ float sm[FEW_WAVES][NR][2];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int64_t rest = blockIdx.x;
-  const int split = (int)(rest % a.splits);
-  const int64_t bh = rest / a.splits;
+  __shared__ uint32_t words[SPAN / 32];
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int split = blockIdx.x % a.splits;
+  const int64_t bh = blockIdx.x / a.splits;
   const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
   const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
   const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
@@ -526,46 +550,84 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
       for (int e = 0; e < N; ++e) q[r][e] *= a.c;
     }
   }
-  const int k_lo = split * a.per_split, k_hi = min(a.Lk, k_lo + a.per_split);
-  for (int k0 = k_lo + wave * KPI * FEW_AHEAD; k0 < k_hi; k0 += FEW_WAVES * KPI * FEW_AHEAD) {
-    typename Vec<T, N>::type kx[FEW_AHEAD], vx[FEW_AHEAD];
+  struct Ahead {
+    typename Vec<T, N>::type k[FEW_AHEAD], v[FEW_AHEAD];
     bool ok[FEW_AHEAD];
-#pragma unroll
-    for (int u = 0; u < FEW_AHEAD; ++u) {
-      const int64_t key = k0 + u * KPI + sub;
-      ok[u] = key < k_hi && (!keep || keep[key]);
-      kx[u] = vx[u] = typename Vec<T, N>::type{};
-      if (ok[u] && act) {
-        kx[u] = *reinterpret_cast<const typename Vec<T, N>::type*>(k + key * a.k_ls + d0);
-        vx[u] = *reinterpret_cast<const typename Vec<T, N>::type*>(v + key * a.v_ls + d0);
-      }
-    }
-#pragma unroll
-    for (int r = 0; r < NR; ++r) {
-      float s[FEW_AHEAD], top = m[r];
-#pragma unroll
-      for (int u = 0; u < FEW_AHEAD; ++u) {
-        float x = 0.f;
-#pragma unroll
-        for (int e = 0; e < N; ++e) x = fmaf(q[r][e], vec_f<T, N>(kx[u], e), x);
-#pragma unroll
-        for (int off = 1; off < LPR; off <<= 1) x += __shfl_xor(x, off, 64);
-        s[u] = ok[u] ? x : -INFINITY;
-        top = fmaxf(top, s[u]);
-      }
-      const float base = top == -INFINITY ? 0.f : top;
-      const float alpha = exp2_fast(m[r] - base);
-      m[r] = top;
-      l[r] *= alpha;
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[r][e] *= alpha;
+  };
+  const int64_t k_lo = (int64_t)split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
+  for (int64_t base = k_lo; base < k_hi; base += SPAN) {
+    __syncthreads();
+    span_words(words, keep, base, k_hi, t, 64 * FEW_WAVES);
+    __syncthreads();
+    const int last = (int)min((int64_t)SPAN, k_hi - base);
+    const auto next = [&](int g) {  // the wave's next group with a key
+      while (g < last && !((words[g >> 5] >> (g & 31)) & GROUP_BITS)) g += STEP;
+      return g;
+    };
+    const auto load = [&](Ahead& x, int g) {
 #pragma unroll
       for (int u = 0; u < FEW_AHEAD; ++u) {
-        const float p = exp2_fast(s[u] - base);
-        l[r] += p;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[r][e] = fmaf(p, vec_f<T, N>(vx[u], e), o[r][e]);
+        const int i = g + u * KPI + sub;
+        x.ok[u] = (words[i >> 5] >> (i & 31)) & 1;
+        x.k[u] = x.v[u] = typename Vec<T, N>::type{};
+        if (x.ok[u] && act) {
+          x.k[u] = *reinterpret_cast<const typename Vec<T, N>::type*>(k + (base + i) * a.k_ls + d0);
+          x.v[u] = *reinterpret_cast<const typename Vec<T, N>::type*>(v + (base + i) * a.v_ls + d0);
+        }
       }
+    };
+    const auto take = [&](const Ahead& x) {
+      float s[NR][FEW_AHEAD];
+#pragma unroll
+      for (int u = 0; u < FEW_AHEAD; ++u) {
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = vec_f<T, N>(x.k[u], e);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          float y = 0.f;
+#pragma unroll
+          for (int e = 0; e < N; ++e) y = fmaf(q[r][e], f[e], y);
+          y = group_add<LPR>(y);
+          s[r][u] = x.ok[u] ? y : -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        float top = m[r];
+#pragma unroll
+        for (int u = 0; u < FEW_AHEAD; ++u) top = fmaxf(top, s[r][u]);
+        const float zero = top == -INFINITY ? 0.f : top;
+        const float alpha = exp2_fast(m[r] - zero);
+        m[r] = top;
+        l[r] *= alpha;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[r][e] *= alpha;
+#pragma unroll
+        for (int u = 0; u < FEW_AHEAD; ++u) l[r] += s[r][u] = exp2_fast(s[r][u] - zero);
+      }
+#pragma unroll
+      for (int u = 0; u < FEW_AHEAD; ++u) {
+        float f[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = vec_f<T, N>(x.v[u], e);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[r][e] = fmaf(s[r][u], f[e], o[r][e]);
+      }
+    };
+    Ahead x, y;
+    int g = next(wave * GROUP);
+    if (g < last) load(x, g);
+    while (g < last) {
+      const int g2 = next(g + STEP);
+      if (g2 < last) load(y, g2);
+      take(x);
+      if (g2 >= last) break;
+      g = next(g2 + STEP);
+      if (g < last) load(x, g);
+      take(y);
     }
   }
 #pragma unroll
@@ -573,8 +635,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
 #pragma unroll
     for (int off = LPR; off < 64; off <<= 1) {
       const float m2 = __shfl_xor(m[r], off, 64), l2 = __shfl_xor(l[r], off, 64);
-      const float top = fmaxf(m[r], m2), base = top == -INFINITY ? 0.f : top;
-      const float w = exp2_fast(m[r] - base), w2 = exp2_fast(m2 - base);
+      const float top = fmaxf(m[r], m2), zero = top == -INFINITY ? 0.f : top;
+      const float w = exp2_fast(m[r] - zero), w2 = exp2_fast(m2 - zero);
       m[r] = top;
       l[r] = l[r] * w + l2 * w2;
 #pragma unroll
@@ -594,11 +656,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < FEW_WAVES; ++w) top = fmaxf(top, sm[w][r][0]);
-    const float base = top == -INFINITY ? 0.f : top;
+    const float zero = top == -INFINITY ? 0.f : top;
     float x = 0.f, sum = 0.f;
 #pragma unroll
     for (int w = 0; w < FEW_WAVES; ++w) {
-      const float f = exp2_fast(sm[w][r][0] - base);
+      const float f = exp2_fast(sm[w][r][0] - zero);
       x += f * so[w][r][d];
       sum += f * sm[w][r][1];
     }
@@ -621,27 +683,27 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
 }
 
 // ---- backward ------------------------------------------------------------------------------------
-// delta[b, h, i] = sum_d dO O.  16 lanes a row.
-template <class T>
+// delta[b, h, i] = sum_d dO O, where dQ, which computes it on its way, is not wanted: two lanes a row,
+// the sums in dQ's order (the same bits).
+template <class T, class M>
 __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);  // (b, i, h)
-  const int c = threadIdx.x & 15;
+  constexpr int N = M::CHUNK / 2;
+  const int64_t row = (int64_t)blockIdx.x * 128 + (threadIdx.x >> 1);  // (b, i, h)
+  const int half = threadIdx.x & 1;
   float s = 0.f;
   const bool in = row < (int64_t)a.B * a.Lq * a.H;
   const int h = (int)(row % a.H);
   const int64_t bi = row / a.H;
   const int i = (int)(bi % a.Lq), b = (int)(bi / a.Lq);
-  if (in && 8 * c < a.D) {
-    float x[8], y[8];
-    load_f<T, 8>(static_cast<const T*>(a.o) + row * a.D + 8 * c, x);
-    load_f<T, 8>(static_cast<const T*>(a.dout) + b * a.do_bs + i * a.do_ls + h * a.do_hs + 8 * c,
-                 y);
+  for (int d = N * half; in && d < a.D; d += M::CHUNK) {
+    float x[N], y[N];
+    load_f<T, N>(static_cast<const T*>(a.o) + row * a.D + d, x);
+    load_f<T, N>(static_cast<const T*>(a.dout) + b * a.do_bs + i * a.do_ls + h * a.do_hs + d, y);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(x[e], y[e], s);
+    for (int e = 0; e < N; ++e) s = fmaf(y[e], x[e], s);
   }
-#pragma unroll
-  for (int off = 1; off < 16; off <<= 1) s += __shfl_xor(s, off, 64);
-  if (in && c == 0) a.delta[((int64_t)b * a.H + h) * a.Lq + i] = s;
+  s += __shfl_xor(s, 1, 64);
+  if (in && half == 0) a.delta[((int64_t)b * a.H + h) * a.Lq + i] = s;
 }
 
 // dQ: WR of the block's waves along the rows (32 each), the others along the staged keys.
@@ -649,7 +711,7 @@ template <class M, int WR>
 constexpr int DQ_KT = sizeof(typename M::elem) == 2 ? (WR == 4 ? 64 : 128) : 32 * (NW / WR);
 
 template <class T, class M, int DP, int WR>
-__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP>)) void xattn_dq_kernel(XArgs a) {
+__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WR>)) void xattn_dq_kernel(XArgs a) {
   typedef typename M::elem E;
   constexpr int KT = DQ_KT<M, WR>, WK = NW / WR, NU = KT / 32 / WK;
   constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
@@ -678,7 +740,21 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP>)) void xattn_dq_kernel(XAr
                           ra.h * a.do_hs,
                       in, a.D, lane);
   const int64_t stat = ((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i;
-  const float lse = in ? a.lse[stat] : -INFINITY, delta = in ? a.delta[stat] : 0.f;
+  const float lse = in ? a.lse[stat] : -INFINITY;
+  float delta = 0.f;
+  {
+    typename M::frag o[NC];
+    load_rows<T, M, DP>(o,
+                        static_cast<const T*>(a.o) + (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) *
+                                                         a.D,
+                        in, a.D, lane);
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < M::CHUNK / 2; ++e) delta = fmaf((float)go[c][e], (float)o[c][e], delta);
+  }
+  delta = halves(delta, [](float x, float y) { return x + y; });
+  if (in && lane < 32 && wk == 0 && j.split == 0) a.delta[stat] = delta;
   // a row without a key (and one that does not exist) has exponents of -inf: P = 0
   const float neg = lse == -INFINITY ? -INFINITY : -lse;
   f32x16 acc[DP / 32] = {};
@@ -762,7 +838,7 @@ template <class M, int WC>
 constexpr int DKV_RT = sizeof(typename M::elem) == 2 && WC == NW ? 64 : 32 * (NW / WC);
 
 template <class T, class M, int DP, int WC>
-__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP>)) void xattn_dkv_kernel(XArgs a) {
+__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WC>)) void xattn_dkv_kernel(XArgs a) {
   typedef typename M::elem E;
   constexpr int RT = DKV_RT<M, WC>, WS = NW / WC, NU = RT / 32 / WS;
   constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
@@ -944,7 +1020,8 @@ Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t lea
   Tiling t;
   t.nw = n <= 32 ? 1 : n <= 64 ? 2 : NW;
   t.tiles = (int)std::max<int64_t>(1, cdiv(n, 32 * t.nw));
-  int64_t s = cdiv(want, std::max<int64_t>(1, heads * t.tiles));
+  const int64_t blocks = std::max<int64_t>(1, heads * t.tiles);
+  int64_t s = 2 * blocks >= want ? 1 : cdiv(want, blocks);
   s = std::max<int64_t>(1, std::min(s, other / least));
   t.per = (int)(cdiv(cdiv(std::max<int64_t>(other, 1), s), unit) * unit);
   t.splits = (int)std::max<int64_t>(1, cdiv(other, t.per));
@@ -965,7 +1042,7 @@ XPlan xattn_plan(const int64_t* dims) {
   XPlan p;
   p.few = R <= FEW_ROWS;
   if (p.few) {
-    p.fwd = tiling(heads, 1, Lk, 1024, 256, 64);
+    p.fwd = tiling(heads, 1, Lk, 512, 1024, 64);
     p.fwd.tiles = 1;
   } else {
     p.fwd = tiling(heads, R, Lk, 256, 256, 128);
@@ -1057,8 +1134,8 @@ int few_rows(const XArgs& a, unsigned blocks, hipStream_t s) {
   constexpr int N = VEC16<T>;
   const dim3 grid(blocks), block(64 * FEW_WAVES);
   if (a.D <= 8 * N) xattn_few_kernel<T, 8, NR><<<grid, block, 0, s>>>(a);
-  else if (a.D <= 16 * N) xattn_few_kernel<T, 16, NR><<<grid, block, 0, s>>>(a);
-  else xattn_few_kernel<T, 32, NR><<<grid, block, 0, s>>>(a);
+  else if (N == 8 || a.D <= 16 * N) xattn_few_kernel<T, 16, NR><<<grid, block, 0, s>>>(a);
+  else if constexpr (N == 4) xattn_few_kernel<T, 32, NR><<<grid, block, 0, s>>>(a);
   MPR_LAUNCHED();
   return MPR_OK;
 }
@@ -1090,22 +1167,9 @@ template <class T>
 int xattn_backward(XArgs a, const XPlan& p, hipStream_t s) {
   typedef typename MmaOf<T>::type M;
   const int64_t rows = (int64_t)a.B * a.Lq * a.H, heads = (int64_t)a.B * a.Hkv;
-  if (rows) {
-    xattn_delta_kernel<T><<<dim3((unsigned)cdiv(rows, 16)), 256, 0, s>>>(a);
+  if (rows && !a.dq) {
+    xattn_delta_kernel<T, M><<<dim3((unsigned)cdiv(rows, 128)), 256, 0, s>>>(a);
     MPR_LAUNCHED();
-  }
-  if (a.Lk && a.dk) {
-    const unsigned blocks = xattn_tile(a, p.dkv);
-    MPR_TRY(by_tile(a.D, p.dkv.nw, [&](auto dp, auto nw) -> int {
-      constexpr int DP = dp, WC = nw;
-      xattn_dkv_kernel<T, M, DP, WC><<<blocks, 64 * NW, 0, s>>>(a);
-      MPR_LAUNCHED();
-      return MPR_OK;
-    }));
-    if (a.splits > 1) {
-      xattn_sum_kernel<T><<<dim3((unsigned)cdiv(heads * a.Lk * a.D, 1024)), 256, 0, s>>>(a, 1);
-      MPR_LAUNCHED();
-    }
   }
   if (rows && a.dq) {
     const unsigned blocks = xattn_tile(a, p.dq);
@@ -1117,6 +1181,19 @@ int xattn_backward(XArgs a, const XPlan& p, hipStream_t s) {
     }));
     if (a.splits > 1) {
       xattn_sum_kernel<T><<<dim3((unsigned)cdiv(heads * a.R * a.D, 1024)), 256, 0, s>>>(a, 0);
+      MPR_LAUNCHED();
+    }
+  }
+  if (a.Lk && a.dk) {
+    const unsigned blocks = xattn_tile(a, p.dkv);
+    MPR_TRY(by_tile(a.D, p.dkv.nw, [&](auto dp, auto nw) -> int {
+      constexpr int DP = dp, WC = nw;
+      xattn_dkv_kernel<T, M, DP, WC><<<blocks, 64 * NW, 0, s>>>(a);
+      MPR_LAUNCHED();
+      return MPR_OK;
+    }));
+    if (a.splits > 1) {
+      xattn_sum_kernel<T><<<dim3((unsigned)cdiv(heads * a.Lk * a.D, 1024)), 256, 0, s>>>(a, 1);
       MPR_LAUNCHED();
     }
   }

@@ -31,6 +31,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -70,7 +72,9 @@ def _rows(t):
 
 def _matrix(t):
     """A matrix whose rows are contiguous and do not overlap."""
-    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    if t.is_contiguous() or (t.stride(1) == 1 and t.stride(0) >= t.shape[1]):
+        return t
+    return t.contiguous()
 
 
 def _tokens(t, device, name: str, below: int, lowest: int):
@@ -78,6 +82,8 @@ def _tokens(t, device, name: str, below: int, lowest: int):
     if not isinstance(t, torch.Tensor) or t.dtype not in _IDS:
         raise TypeError(f"{name}: an int32 or int64 tensor is needed, got "
                         f"{t.dtype if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if t.is_cuda and t.device == device:
+        return t if t.is_contiguous() else t.contiguous()
     if t.device.type == "cpu":
         if t.numel() and (int(t.max()) >= below or int(t.min()) < lowest):
             raise IndexError(f"{name}: values from {int(t.min())} to {int(t.max())}, "
@@ -86,41 +92,58 @@ def _tokens(t, device, name: str, below: int, lowest: int):
         raise ValueError(f"{name}: on {t.device}, needed on {device} (or the host)")
     if device.type != "cuda":
         raise ValueError(f"{name}: libmpr runs on a GPU, the operands are on {device}")
-    if t.device == device:
-        return t.contiguous()
     with torch.cuda.device(device):
         return _lib.to_device_async(t, device).contiguous()
 
 
+@lru_cache(maxsize=4096)
 def _i64(*vals):
+    """The sizes or strides as a C array (read only: shared between calls)."""
     return (ctypes.c_int64 * len(vals))(*vals)
 
 
 def _call(device, name: str, *args) -> None:
     """The library call on the current stream of `device`."""
-    stream = ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, stream)
+    i = device.index
+    if torch._C._cuda_getDevice() == i:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
     else:
-        with torch.cuda.device(device):
-            _lib.call(name, *args, stream)
+        with torch.cuda.device(i):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(i))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+@lru_cache(maxsize=4096)
+def _bytes(name: str, *sizes) -> int:
+    """The size that a workspace entry answers for these sizes."""
+    n = ctypes.c_int64()
+    _lib.call(name, *sizes, ctypes.byref(n))
+    return n.value
 
 
 def _workspace(nbytes: int, device):
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
 
 
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def _first_order(backward):
+    """``once_differentiable``, entered only where the gradient is asked for with a graph."""
+    once = once_differentiable(backward)
+
+    def wrapper(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return wrapper
 
 
 # ---- embedding -----------------------------------------------------------------------------------
 def _embed_fwd(weight, ids, scale):
-    w = _matrix(weight.detach())
+    w = _matrix(weight)
     V, d = w.shape
     out = torch.empty((*ids.shape, d), dtype=w.dtype, device=w.device)
-    _call(w.device, "mpr_embed_lookup", _lib.ptr(w), _DTYPES[w.dtype], V, w.stride(0),
-          _lib.ptr(ids), _IDS[ids.dtype], ids.numel(), d, scale, _lib.ptr(out))
+    _call(w.device, "mpr_embed_lookup", _ptr(w), _DTYPES[w.dtype], V, w.stride(0),
+          _ptr(ids), _IDS[ids.dtype], ids.numel(), d, scale, _ptr(out))
     return out
 
 
@@ -133,18 +156,17 @@ class _Embed(torch.autograd.Function):
         return _embed_fwd(weight, ids, scale)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         (ids,), ((V, d), dtype), (scale, pad) = ctx.saved_tensors, ctx.table, ctx.args
         n, code = ids.numel(), _DTYPES[dtype]
-        dout = _matrix(dout.reshape(n, d))
+        dout = _matrix(dout if dout.dim() == 2 else dout.reshape(n, d))
         dw = torch.empty((V, d), dtype=dtype, device=dout.device)
-        nbytes = ctypes.c_int64()
-        _lib.call("mpr_embed_grad_workspace", code, n, V, d, ctypes.byref(nbytes))
-        ws = _workspace(nbytes.value, dout.device)
-        _call(dout.device, "mpr_embed_grad", _lib.ptr(dout), code, dout.stride(0),
-              _lib.ptr(ids), _IDS[ids.dtype], n, V, d, scale, pad, _lib.ptr(dw), _lib.ptr(ws),
-              nbytes.value)
+        nbytes = _bytes("mpr_embed_grad_workspace", code, n, V, d)
+        ws = _workspace(nbytes, dout.device)
+        _call(dout.device, "mpr_embed_grad", _ptr(dout), code, dout.stride(0),
+              _ptr(ids), _IDS[ids.dtype], n, V, d, scale, pad, _ptr(dw), _ptr(ws),
+              nbytes)
         return dw, None, None, None
 
 
@@ -157,7 +179,7 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
     lies on the device cannot be refused without waiting for the GPU: it gives a row of NaN and no
     gradient."""
     _floating(weight, "embed weight")
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+    if weight.dim() != 2 or weight.numel() == 0:
         raise ValueError(f"embed: a table [V, d] is needed, got {tuple(weight.shape)}")
     V = weight.shape[0]
     pad = -1
@@ -167,7 +189,7 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
         pad = int(padding_idx) % V
     scale = float(scale)
     ids = _tokens(ids, weight.device, "embed ids", V, 0)
-    if _wants_grad(weight):
+    if weight.requires_grad and torch.is_grad_enabled():
         return _Embed.apply(weight, ids, scale, pad)
     return _embed_fwd(weight, ids, scale)
 
@@ -175,7 +197,7 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
 # ---- cross attention -----------------------------------------------------------------------------
 def _xattn_dims(q, k):
     B, Lq, H, D = q.shape
-    return _i64(B, H, k.shape[2], Lq, k.shape[1], D)
+    return B, H, k.shape[2], Lq, k.shape[1], D
 
 
 def _xattn_strides(q, k, v, keep, dout=None):
@@ -184,9 +206,10 @@ def _xattn_strides(q, k, v, keep, dout=None):
     return _i64(*s, *(dout.stride()[:3] if dout is not None else (0, 0, 0)))
 
 
-def _xattn_bytes(dims, code):
+@lru_cache(maxsize=4096)
+def _xattn_bytes(code, *dims):
     fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
-    _lib.call("mpr_xattn_workspace", dims, code, ctypes.byref(fwd), ctypes.byref(bwd))
+    _lib.call("mpr_xattn_workspace", _i64(*dims), code, ctypes.byref(fwd), ctypes.byref(bwd))
     return fwd.value, bwd.value
 
 
@@ -197,10 +220,10 @@ def _xattn_fwd(q, k, v, keep, scale, want_lse):
     if want_lse:
         B, Lq, H, _ = q.shape
         lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
-    nbytes, _ = _xattn_bytes(dims, code)
+    nbytes, _ = _xattn_bytes(code, *dims)
     ws = _workspace(nbytes, q.device)
-    _call(q.device, "mpr_xattn_fwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(keep), code,
-          dims, _xattn_strides(q, k, v, keep), scale, _lib.ptr(out), _lib.ptr(lse), _lib.ptr(ws),
+    _call(q.device, "mpr_xattn_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(keep), code,
+          _i64(*dims), _xattn_strides(q, k, v, keep), scale, _ptr(out), _ptr(lse), _ptr(ws),
           nbytes)
     return out, lse
 
@@ -208,14 +231,14 @@ def _xattn_fwd(q, k, v, keep, scale, want_lse):
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, keep, scale):
-        q, k, v = (_rows(t.detach()) for t in (q, k, v))
+        q, k, v = _rows(q), _rows(k), _rows(v)
         out, lse = _xattn_fwd(q, k, v, keep, scale, True)
         ctx.save_for_backward(q, k, v, keep, out, lse)
         ctx.scale = scale
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dout):
         q, k, v, keep, out, lse = ctx.saved_tensors
         dout = _rows(dout)
@@ -226,12 +249,12 @@ class _CrossAttention(torch.autograd.Function):
             return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
         dq = like(q, need_q)
         dk, dv = (like(t, need_k or need_v) for t in (k, v))
-        _, nbytes = _xattn_bytes(dims, code)
+        _, nbytes = _xattn_bytes(code, *dims)
         ws = _workspace(nbytes, q.device)
-        _call(q.device, "mpr_xattn_bwd", _lib.ptr(q), _lib.ptr(k), _lib.ptr(v), _lib.ptr(keep),
-              code, dims, _xattn_strides(q, k, v, keep, dout), ctx.scale, _lib.ptr(out),
-              _lib.ptr(lse), _lib.ptr(dout), _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv),
-              _lib.ptr(ws), nbytes)
+        _call(q.device, "mpr_xattn_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(keep),
+              code, _i64(*dims), _xattn_strides(q, k, v, keep, dout), ctx.scale, _ptr(out),
+              _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv),
+              _ptr(ws), nbytes)
         return dq, dk if need_k else None, dv if need_v else None, None, None
 
 
@@ -277,10 +300,9 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
     if key_mask is not None:
         keep = key_mask if key_mask.dtype == torch.bool else key_mask != 0
         keep = _rows(keep.detach().expand(B, Lk)).view(torch.uint8)
-    if _wants_grad(q, k, v):
+    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
         return _CrossAttention.apply(q, k, v, keep, scale)
-    return _xattn_fwd(_rows(q.detach()), _rows(k.detach()), _rows(v.detach()), keep, scale,
-                      False)[0]
+    return _xattn_fwd(_rows(q), _rows(k), _rows(v), keep, scale, False)[0]
 
 
 # ---- log-probabilities and the preference loss -----------------------------------------------------
@@ -308,35 +330,34 @@ def _logps_fwd(logits, labels, pair):
     logps, stat = f32(S), f32(S, T, 2)
     loss, dlogps = (f32(), f32(S)) if pair else (None, None)
     ref, beta, smooth = pair or (None, 0.0, 0.0)
-    nbytes = ctypes.c_int64()
-    _lib.call("mpr_logps_workspace", S, T, V, ctypes.byref(nbytes))
-    ws = _workspace(nbytes.value, dev)
-    _call(dev, "mpr_logps_fwd", _lib.ptr(logits), _DTYPES[logits.dtype], S, T, V,
-          logits.stride(0), logits.stride(1), _lib.ptr(labels), _IDS[labels.dtype], T,
-          _lib.ptr(logps), _lib.ptr(stat), _lib.ptr(ref), beta, smooth, _lib.ptr(loss),
-          _lib.ptr(dlogps), _lib.ptr(ws), nbytes.value)
+    nbytes = _bytes("mpr_logps_workspace", S, T, V)
+    ws = _workspace(nbytes, dev)
+    _call(dev, "mpr_logps_fwd", _ptr(logits), _DTYPES[logits.dtype], S, T, V,
+          logits.stride(0), logits.stride(1), _ptr(labels), _IDS[labels.dtype], T,
+          _ptr(logps), _ptr(stat), _ptr(ref), beta, smooth, _ptr(loss),
+          _ptr(dlogps), _ptr(ws), nbytes)
     return logps, stat, loss, dlogps
 
 
 def _logps_bwd(logits, labels, stat, dlogps, mult):
     S, T, V = logits.shape
     dx = torch.empty((S, T, V), dtype=logits.dtype, device=logits.device)
-    _call(logits.device, "mpr_logps_bwd", _lib.ptr(logits), _DTYPES[logits.dtype], S, T, V,
-          logits.stride(0), logits.stride(1), _lib.ptr(labels), _IDS[labels.dtype], T,
-          _lib.ptr(stat), _lib.ptr(dlogps), _lib.ptr(mult), _lib.ptr(dx))
+    _call(logits.device, "mpr_logps_bwd", _ptr(logits), _DTYPES[logits.dtype], S, T, V,
+          logits.stride(0), logits.stride(1), _ptr(labels), _IDS[labels.dtype], T,
+          _ptr(stat), _ptr(dlogps), _ptr(mult), _ptr(dx))
     return dx
 
 
 class _SequenceLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels):
-        logits = _rows(logits.detach())
+        logits = _rows(logits)
         logps, stat, _, _ = _logps_fwd(logits, labels, None)
         ctx.save_for_backward(logits, labels, stat)
         return logps
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dlogps):
         logits, labels, stat = ctx.saved_tensors
         return _logps_bwd(logits, labels, stat, dlogps.contiguous(), None), None
@@ -345,14 +366,14 @@ class _SequenceLogps(torch.autograd.Function):
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref, beta, smooth):
-        logits = _rows(logits.detach())
+        logits = _rows(logits)
         logps, stat, loss, dlogps = _logps_fwd(logits, labels, (ref, beta, smooth))
         ctx.save_for_backward(logits, labels, stat, dlogps)
         ctx.mark_non_differentiable(logps)
         return loss, logps
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dloss, _):
         logits, labels, stat, dlogps = ctx.saved_tensors
         return (_logps_bwd(logits, labels, stat, dlogps, dloss.contiguous()), None, None, None,
@@ -369,9 +390,9 @@ def sequence_logps(logits, labels):
     side of ``preference_loss``."""
     _logps_shapes(logits, labels, "sequence_logps")
     labels = _label_ids(logits, labels, "sequence_logps")
-    if _wants_grad(logits):
+    if logits.requires_grad and torch.is_grad_enabled():
         return _SequenceLogps.apply(logits, labels)
-    return _logps_fwd(_rows(logits.detach()), labels, None)[0]
+    return _logps_fwd(_rows(logits), labels, None)[0]
 
 
 def preference_loss(logits, labels, ref_logps, beta: float = 0.1, label_smoothing: float = 0.0):
@@ -399,17 +420,15 @@ def preference_loss(logits, labels, ref_logps, beta: float = 0.1, label_smoothin
         raise ValueError(f"preference_loss: label_smoothing {smooth} (0 to 0.5)")
     labels = _label_ids(logits, labels, "preference_loss")
     ref = ref_logps.detach().to(torch.float32).contiguous()
-    if _wants_grad(logits):
+    if logits.requires_grad and torch.is_grad_enabled():
         return _PreferenceLoss.apply(logits, labels, ref, beta, smooth)
-    logps, _, loss, _ = _logps_fwd(_rows(logits.detach()), labels, (ref, beta, smooth))
+    logps, _, loss, _ = _logps_fwd(_rows(logits), labels, (ref, beta, smooth))
     return loss, logps
 
 
 # ---- gradient clipping ---------------------------------------------------------------------------
 def _dense(t) -> bool:
     """Whether the tensor fills its memory without gaps or repeats (in whatever order)."""
-    if t.is_contiguous():
-        return True
     want = 1
     for n, s in sorted(zip(t.shape, t.stride()), key=lambda p: p[1]):
         if n != 1:
@@ -419,45 +438,64 @@ def _dense(t) -> bool:
     return True
 
 
-def _clip(grads, out, max_norm, eps, what):
-    grads = list(grads)
-    if out is not None and len(out) != len(grads):
-        raise ValueError(f"{what}: {len(grads)} gradients and {len(out)} outputs")
-    desc = (ctypes.c_int64 * (5 * len(grads)))()
-    device = None
+def _codes(tensors, what):
+    try:  # hundreds of tensors a call: the names of what is wrong are made only then
+        return [_DTYPES[t.dtype] for t in tensors]
+    except (KeyError, AttributeError):
+        return [_floating(t, f"{what} {i}") for i, t in enumerate(tensors)]
+
+
+def _check_grads(grads, what):
+    """(device, dtype codes) of the gradients, or the refusal of the first that will not do."""
+    codes = _codes(grads, what + " gradient")
+    device, index = grads[0].device, grads[0].get_device()
     for i, g in enumerate(grads):
-        code = _floating(g, f"{what} gradient {i}")
-        device = device or g.device
-        if g.device != device or g.layout is not torch.strided:
+        if g.get_device() != index or g.layout is not torch.strided:
             raise ValueError(f"{what}: gradient {i} is a {g.layout} tensor on {g.device}, needed "
                              f"dense on {device}")
-        if not _dense(g):
+        if not (g.is_contiguous() or _dense(g)):
             raise ValueError(f"{what}: gradient {i} {tuple(g.shape)} with strides {g.stride()} "
                              "leaves gaps in its memory (clip a .contiguous() copy)")
-        o = 5 * i
-        desc[o], desc[o + 1], desc[o + 2] = g.data_ptr(), g.numel(), code
-        if max_norm is None:
-            continue
-        if out is None:
-            desc[o + 3], desc[o + 4] = desc[o], code
-            continue
-        t = out[i]
-        desc[o + 4] = _floating(t, f"{what} output {i}")
-        if t.device != device or t.shape != g.shape:
+    return device, codes
+
+
+def _check_outs(grads, out, device, what):
+    if len(out) != len(grads):
+        raise ValueError(f"{what}: {len(grads)} gradients and {len(out)} outputs")
+    codes = _codes(out, what + " output")
+    index = grads[0].get_device()
+    for i, (g, t) in enumerate(zip(grads, out)):
+        if t.get_device() != index or t.shape != g.shape:
             raise ValueError(f"{what}: output {i} is {tuple(t.shape)} on {t.device}, its gradient "
                              f"{tuple(g.shape)} on {device}")
-        if t.stride() != g.stride() and not (t.is_contiguous() and g.is_contiguous()):
+        if not (t.is_contiguous() and g.is_contiguous()) and t.stride() != g.stride():
             raise ValueError(f"{what}: output {i} is laid out otherwise than its gradient")
-        desc[o + 3] = t.data_ptr()
-    if device is None:
+    return codes
+
+
+def _clip(grads, out, max_norm, eps, what):
+    n = len(grads)
+    if n == 0:
+        if out:
+            raise ValueError(f"{what}: 0 gradients and {len(out)} outputs")
         return torch.zeros(())
+    device, codes = _check_grads(grads, what)
+    into = codes if out is None else _check_outs(grads, out, device, what)
     _on_gpu(grads[0], what)
+    table = array("q", bytes(40 * n))  # n x {pointer, values, type, output pointer, its type}
+    table[0::5] = array("q", [g.data_ptr() for g in grads])
+    table[1::5] = array("q", [g.numel() for g in grads])
+    table[2::5] = array("q", codes)
+    if max_norm is not None:
+        table[3::5] = table[0::5] if out is None else array("q", [t.data_ptr() for t in out])
+        table[4::5] = array("q", into)
+    desc = (ctypes.c_int64 * (5 * n)).from_buffer(table)
     norm = torch.empty((), dtype=torch.float32, device=device)
     nbytes = ctypes.c_int64()
-    _lib.call("mpr_clip_workspace", len(grads), desc, ctypes.byref(nbytes))
+    _lib.call("mpr_clip_workspace", n, desc, ctypes.byref(nbytes))
     ws = _workspace(nbytes.value, device)
-    _call(device, "mpr_clip_grads", len(grads), desc, max_norm or 0.0, eps, _lib.ptr(norm),
-          _lib.ptr(ws), nbytes.value)
+    _call(device, "mpr_clip_grads", n, desc, max_norm or 0.0, eps, _ptr(norm), _ptr(ws),
+          nbytes.value)
     return norm
 
 
@@ -465,7 +503,7 @@ def _clip(grads, out, max_norm, eps, what):
 def grad_norm(grads):
     """The L2 norm of all values of the tensors together (a float32 scalar on their device; 0 on the
     host for none).  Squares are summed in 64 bits."""
-    return _clip(grads, None, None, 0.0, "grad_norm")
+    return _clip(list(grads), None, None, 0.0, "grad_norm")
 
 
 @torch.no_grad()
