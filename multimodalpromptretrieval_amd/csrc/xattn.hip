@@ -8,9 +8,9 @@
 // size Lq x Lk is kept.  A row of all shared heads of a group lies in one tile, so K and V are read
 // once for the group and dK, dV sum the heads in registers: no atomics, the same bits every run.
 //
-// Matrix products: bf16 inputs on v_mfma_f32_32x32x16_bf16, float and half inputs on
-// v_mfma_f32_32x32x2_f32 (exact fp32 products; half gradients would leave half's range as matrix
-// operands).  The products are arranged so that a tile's scores come out of the matrix core in the
+// Matrix products: bf16 inputs on v_mfma_f32_32x32x16_bf16, float inputs on v_mfma_f32_32x32x2_f32
+// (exact fp32 products).  Half is for single tokens only: as matrix operands, half gradients would
+// leave half's range, so the caller computes them in float.  The products are arranged so that a tile's scores come out of the matrix core in the
 // lane order in which the next product takes them (scores transposed: lane = row, registers =
 // keys): probabilities go from one product to the next in registers, never through LDS.  P and dS
 // are rounded to bf16 as operands of the second products (half a step, 2^-9 relative each), as the
@@ -33,6 +33,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr int NW = 4;  // waves of a block (of the tiled kernels)
 
 struct XArgs {
   const void *q, *k, *v, *dout, *o;
@@ -131,6 +132,77 @@ __device__ __forceinline__ typename M::frag row_frag(const typename M::elem* p, 
       p + r * DP + (x ^ (2 * c & 7)) * PIECE<M> + r0 * DP + (2 * c & ~7) * PIECE<M>);
 }
 
+// The compiler keeps the order across this point.  Below, operands are read from LDS AHEAD calls before
+// the matrix core takes them, in the order written: left to itself it reads each where it is used,
+// and every call waits out LDS's latency.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+constexpr int AHEAD = 4;
+
+// acc += the chunks' products of the LDS rows r0 .. r0 + 31 with f (one or two such sums side by
+// side: neighbouring calls do not wait for each other's result)
+template <class M, int DP>
+__device__ __forceinline__ void rows_mma(const typename M::elem* p, int r0,
+                                         const typename M::frag (&f)[DP / M::CHUNK], f32x16& acc,
+                                         int lane) {
+  constexpr int NC = DP / M::CHUNK, A = AHEAD < NC ? AHEAD : NC;
+  typename M::frag x[A];
+#pragma unroll
+  for (int c = 0; c < A; ++c) x[c] = row_frag<M, DP>(p, r0, c, lane);
+  in_order();
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    acc = M::mma(x[c % A], f[c], acc);
+    if (c + A < NC) x[c % A] = row_frag<M, DP>(p, r0, c + A, lane);
+    in_order();
+  }
+}
+template <class M, int DP, class F1, class F2>
+__device__ __forceinline__ void rows_mma2(const typename M::elem* p1, const typename M::elem* p2,
+                                          int r0, F1 f1, F2 f2, f32x16& acc1, f32x16& acc2,
+                                          int lane) {
+  constexpr int NC = DP / M::CHUNK, A = DP == 128 ? AHEAD / 2 : AHEAD;
+  typename M::frag x[A], y[A], g[A];
+#pragma unroll
+  for (int c = 0; c < A; ++c) {
+    x[c] = row_frag<M, DP>(p1, r0, c, lane);
+    y[c] = row_frag<M, DP>(p2, r0, c, lane);
+    g[c] = f2(c);
+  }
+  in_order();
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    acc1 = M::mma(x[c % A], f1(c), acc1);
+    acc2 = M::mma(y[c % A], g[c % A], acc2);
+    if (c + A < NC) {
+      x[c % A] = row_frag<M, DP>(p1, r0, c + A, lane);
+      y[c % A] = row_frag<M, DP>(p2, r0, c + A, lane);
+      g[c % A] = f2(c + A);
+    }
+    in_order();
+  }
+}
+// acc[d] += (columns 32 d .. of LDS rows k0 .. k0 + 31, transposed) x s, s a result of 32 x 32
+template <class M, int DP>
+__device__ __forceinline__ void cols_mma(const typename M::elem* p, int k0, const f32x16& s,
+                                         f32x16 (&acc)[DP / 32], int lane) {
+  constexpr int ND = DP / 32, PC = 32 / M::CHUNK, NI = ND * PC, A = AHEAD < NI ? AHEAD : NI;
+  typename M::frag x[A], f[PC];
+  const auto get = [&](int i) {
+    return M::template col<DP>(p, k0 + i / ND * M::CHUNK, i % ND * 32, lane);
+  };
+#pragma unroll
+  for (int i = 0; i < A; ++i) x[i] = get(i);
+#pragma unroll
+  for (int c = 0; c < PC; ++c) f[c] = M::pack(s, c);
+  in_order();
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    acc[i % ND] = M::mma(x[i % A], f[i / ND], acc[i % ND]);
+    if (i + A < NI) x[i % A] = get(i + A);
+    in_order();
+  }
+}
+
 // the row (0 .. 31) that result register r of this lane's half holds
 __device__ __forceinline__ int acc_row(int r, int lane) {
   return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
@@ -145,39 +217,39 @@ __device__ __forceinline__ float halves(float x, F f) {
 }
 
 // ---- staging -------------------------------------------------------------------------------------
-// A tile of ROWS rows on its way from memory to LDS: load() starts the reads of rows [r0, r0 +
-// ROWS) (those past `end` and columns past D read nothing), put() writes them as M's elements, zeros
-// in place of what was not read and of rows whose bit in `words` is 0.  at(r): the row's first
-// element.  Loads are issued a tile ahead and wait in registers while the tile before is computed.
-template <class T, class M, int DP, int ROWS, int THREADS>
-struct Stage {
-  typedef typename M::elem E;
-  static constexpr int N = PIECE<M>, CH = DP / N, CNT = ROWS * CH / THREADS;
-  static_assert(ROWS * CH % THREADS == 0, "whole pieces a thread");
-  typename Vec<T, N>::type x[CNT];
-  template <class At>
-  __device__ __forceinline__ void load(int64_t r0, int64_t end, int D, At at, int t) {
+// A tile of ROWS rows from memory straight to LDS (no registers in between): starts the reads; they
+// have landed after landed() and a barrier.  A wave's call writes 64 neighbouring pieces, so the
+// permutation of a row's pieces is in what each lane reads.  Rows past `last` read that row and
+// pieces past column D the row's first: what they hold meets only zeros (patch(), or the register
+// operand's own zero columns).  at(r): the row's first element.
+template <class E, int DP, int ROWS, class At>
+__device__ __forceinline__ void stage(E* lds, int64_t r0, int64_t last, int D, At at, int wave,
+                                      int lane) {
+  constexpr int N = 16 / (int)sizeof(E), CH = DP / N, CNT = ROWS * CH / (64 * NW);
+  static_assert(ROWS * CH % (64 * NW) == 0, "whole calls a wave");
 #pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int p = i * THREADS + t, r = p / CH, c = (p % CH) * N;
-      x[i] = typename Vec<T, N>::type{};
-      if (r0 + r < end && c < D)
-        x[i] = *reinterpret_cast<const typename Vec<T, N>::type*>(at(r0 + r) + c);
-    }
+  for (int i = 0; i < CNT; ++i) {
+    const int first = (i * NW + wave) * 64, slot = first + lane, r = slot / CH;
+    int c = ((slot % CH) ^ swz(r)) * N;
+    c = c < D ? c : 0;
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(at(min(r0 + r, last)) + c),
+        (__attribute__((address_space(3))) void*)(lds + first * N), 16, 0, 0);
   }
-  __device__ __forceinline__ void put(E* lds, const uint32_t* words, int t) {
-    typedef E piece __attribute__((ext_vector_type(N)));
-#pragma unroll
-    for (int i = 0; i < CNT; ++i) {
-      const int p = i * THREADS + t, r = p / CH, c = p % CH;
-      const bool on = !words || (words[r >> 5] >> (r & 31)) & 1;
-      piece v;
-#pragma unroll
-      for (int e = 0; e < N; ++e) v[e] = on ? (E)x[i][e] : (E)0.f;
-      *reinterpret_cast<piece*>(lds + r * DP + ((c ^ swz(r)) * N)) = v;
-    }
+}
+// this wave's reads into LDS are done (before the barrier that shows them to the others)
+__device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// zeros in the rows of a staged tile whose bit is 0
+template <class E, int DP, int ROWS>
+__device__ __forceinline__ void patch(E* lds, const uint32_t* words, int t) {
+  constexpr int N = 16 / (int)sizeof(E), CH = DP / N;
+  for (int p = t; p < ROWS * CH; p += 64 * NW) {
+    const int r = p / CH;
+    if (!((words[r >> 5] >> (r & 31)) & 1))
+      *reinterpret_cast<f32x4*>(lds + p * N) = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-};
+}
 
 // a wave's 32 rows as second operands in registers: frag c = contraction chunk c of row lane & 31
 template <class T, class M, int DP>
@@ -286,31 +358,101 @@ __device__ __forceinline__ Job job_of(const XArgs& a) {
   return j;
 }
 
-constexpr int NW = 4;  // waves of a block
-// Waves a SIMD is to hold (what the registers are shared by).
-template <class M, int DP>
-constexpr int FWD_OCC = sizeof(typename M::elem) == 2 ? (DP == 64 ? 3 : 2) : (DP == 64 ? 2 : 1);
-template <class M, int DP, int W>
-constexpr int BWD_OCC = DP == 64 && (sizeof(typename M::elem) == 2 || W == NW) ? 2 : 1;
-// The block's waves: WR of them along the rows (32 each), NW / WR along the staged keys.
-// KT keys are staged at a time.
-template <class M, int WR>
-constexpr int FWD_KT = sizeof(typename M::elem) == 2 ? (WR == 4 ? 64 : 128) : 32 * (NW / WR);
+// The block's waves: WR of them along the rows (32 each), NW / WR along the staged keys, KT at a time.
+// OCC: waves a SIMD is to hold, which is what its registers are shared by.  Tiles are staged into one
+// buffer while the other is computed, where two fit.
+template <class M, int DP, int WR>
+struct Shape {
+  typedef typename M::elem E;
+  static constexpr bool HALF = sizeof(E) == 2;
+  static constexpr int WK = NW / WR;
+  static constexpr int KT = HALF && WR == NW ? 64 : 32 * WK;
+  static constexpr int NU = KT / 32 / WK;  // a wave's 32-key products in a tile
+  static constexpr int FWD_OCC = HALF ? (DP == 64 ? 3 : 2) : (DP == 64 ? 2 : 1);
+  static constexpr int BWD_OCC = HALF || (DP == 64 && WR == NW) ? 2 : 1;
+  static constexpr int TILE = KT * DP;  // elements of K, and of V
+  static constexpr int BUFS = 4 * TILE * (int)sizeof(E) <= 131072 ? 2 : 1;
+  static constexpr int JOIN = (NW - WR) * (DP * 32 + 128) * 4;  // bytes, at the end
+  static constexpr int BYTES = 2 * TILE * (int)sizeof(E) > JOIN ? 2 * TILE * (int)sizeof(E) : JOIN;
+};
+
+// Runs over the live tiles of the block's keys [k_lo, k_hi): for each, compute(K, V, the tile's
+// words).  ZERO_K: masked keys' rows of K become zeros as V's do.
+template <class T, class M, int DP, int WR, bool ZERO_K, class KAt, class VAt, class F>
+__device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* words,
+                                          const uint8_t* keep, int64_t k_lo, int64_t k_hi, int D,
+                                          KAt k_at, VAt v_at, int t, int wave, int lane,
+                                          F compute) {
+  typedef Shape<M, DP, WR> S;
+  typedef typename M::elem E;
+  constexpr int KT = S::KT;
+  for (int64_t base = k_lo; base < k_hi; base += SPAN) {
+    __syncthreads();
+    span_words(words, keep, base, k_hi, t, 64 * NW);
+    __syncthreads();
+    const int last = (int)min((int64_t)SPAN, k_hi - base);
+    const auto load = [&](char* lds, int at) {
+      E* k = reinterpret_cast<E*>(lds);
+      stage<E, DP, KT>(k, base + at, k_hi - 1, D, k_at, wave, lane);
+      stage<E, DP, KT>(k + S::TILE, base + at, k_hi - 1, D, v_at, wave, lane);
+    };
+    const auto take = [&](char* lds, int at) {
+      E* k = reinterpret_cast<E*>(lds);
+      uint32_t all = ~0u;
+#pragma unroll
+      for (int u = 0; u < KT / 32; ++u) all &= words[at / 32 + u];
+      if (all != ~0u) {  // the same for every wave
+        if (ZERO_K) patch<E, DP, KT>(k, words + at / 32, t);
+        patch<E, DP, KT>(k + S::TILE, words + at / 32, t);
+        __syncthreads();
+      }
+      compute(k, k + S::TILE, words + at / 32);
+    };
+    int at = next_tile<KT>(words, 0, last);
+    if (at >= last) continue;
+    load(lds0, at);
+    landed();
+    __syncthreads();
+    if constexpr (S::BUFS == 2) {
+      for (;;) {
+        const int b = next_tile<KT>(words, at + KT, last);
+        if (b < last) load(lds1, b);
+        take(lds0, at);
+        if (b >= last) break;
+        landed();
+        __syncthreads();
+        at = next_tile<KT>(words, b + KT, last);
+        if (at < last) load(lds0, at);
+        take(lds1, b);
+        if (at >= last) break;
+        landed();
+        __syncthreads();
+      }
+    } else {
+      for (;;) {
+        take(lds0, at);
+        at = next_tile<KT>(words, at + KT, last);
+        if (at >= last) break;
+        __syncthreads();
+        load(lds0, at);
+        landed();
+        __syncthreads();
+      }
+    }
+  }
+}
 
 // ---- forward -------------------------------------------------------------------------------------
 // The running maximum follows the scores only when they pass it by more than 8 (in base 2): until
 // then exponentials up to 2^8 share the old base, and the sums need no rescaling.
 template <class T, class M, int DP, int WR>
-__global__ __launch_bounds__(64 * NW, (FWD_OCC<M, DP>)) void xattn_fwd_kernel(XArgs a) {
+__global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fwd_kernel(XArgs a) {
+  typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
-  constexpr int KT = FWD_KT<M, WR>, WK = NW / WR, NU = KT / 32 / WK;
-  constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
-  constexpr int TILE_BYTES = 2 * KT * DP * (int)sizeof(E);
-  constexpr int JOIN_BYTES = (NW - WR) * (DP * 32 + 128) * 4;
-  __shared__ __align__(16) char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
+  constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  __shared__ __align__(16) char lds[S::BYTES];
+  __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
   __shared__ uint32_t words[SPAN / 32];
-  E* ks = reinterpret_cast<E*>(lds);
-  E* vs = ks + KT * DP;
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
   const Job j = job_of(a);
@@ -328,45 +470,23 @@ __global__ __launch_bounds__(64 * NW, (FWD_OCC<M, DP>)) void xattn_fwd_kernel(XA
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;  // of the unscaled scores
   const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
-  Stage<T, M, DP, KT, 64 * NW> sk, sv;
-  for (int64_t base = k_lo; base < k_hi; base += SPAN) {
-    __syncthreads();
-    span_words(words, keep, base, k_hi, t, 64 * NW);
-    __syncthreads();
-    const int last = (int)min((int64_t)SPAN, k_hi - base);
-    int next = next_tile<KT>(words, 0, last);
-    if (next < last) {
-      sk.load(base + next, k_hi, a.D, k_at, t);
-      sv.load(base + next, k_hi, a.D, v_at, t);
-    }
-    while (next < last) {
-      const int cur = next;
-      __syncthreads();
-      sk.put(ks, nullptr, t);
-      sv.put(vs, words + cur / 32, t);
-      __syncthreads();
-      next = next_tile<KT>(words, cur + KT, last);
-      if (next < last) {
-        sk.load(base + next, k_hi, a.D, k_at, t);
-        sv.load(base + next, k_hi, a.D, v_at, t);
-      }
+  for_tiles<T, M, DP, WR, false>(lds, lds1, words, keep, k_lo, k_hi, a.D, k_at, v_at, t, wave, lane,
+                                 [&](const E* ks, const E* vs, const uint32_t* on) {
       const int u0 = wk * NU;
       uint32_t bits[NU], any = 0, all = ~0u;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        bits[u] = __builtin_amdgcn_readfirstlane(words[cur / 32 + u0 + u]);
+        bits[u] = __builtin_amdgcn_readfirstlane(on[u0 + u]);
         any |= bits[u];
         all &= bits[u];
       }
-      if (any == 0) continue;  // this wave's keys (its barriers come with the next tile)
+      if (any == 0) return;  // none of this wave's keys
       f32x16 s[NU];
       float top = m;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
         s[u] = f32x16{};
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-          s[u] = M::mma(row_frag<M, DP>(ks, 32 * (u0 + u), c, lane), q[c], s[u]);
+        rows_mma<M, DP>(ks, 32 * (u0 + u), q, s[u], lane);
       }
       if (all != ~0u) {
 #pragma unroll
@@ -398,17 +518,8 @@ __global__ __launch_bounds__(64 * NW, (FWD_OCC<M, DP>)) void xattn_fwd_kernel(XA
         }
       l += sum[0] + sum[1];
 #pragma unroll
-      for (int u = 0; u < NU; ++u)
-#pragma unroll
-        for (int c = 0; c < PC; ++c) {
-          const typename M::frag p = M::pack(s[u], c);
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d)
-            acc[d] = M::mma(M::template col<DP>(vs, 32 * (u0 + u) + c * M::CHUNK, 32 * d, lane), p,
-                            acc[d]);
-        }
-    }
-  }
+      for (int u = 0; u < NU; ++u) cols_mma<M, DP>(vs, 32 * (u0 + u), s[u], acc, lane);
+  });
   l = halves(l, [](float x, float y) { return x + y; });
   if constexpr (WK > 1) {  // the waves along the keys
     __syncthreads();
@@ -707,20 +818,14 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
 }
 
 // dQ: WR of the block's waves along the rows (32 each), the others along the staged keys.
-template <class M, int WR>
-constexpr int DQ_KT = sizeof(typename M::elem) == 2 ? (WR == 4 ? 64 : 128) : 32 * (NW / WR);
-
 template <class T, class M, int DP, int WR>
-__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WR>)) void xattn_dq_kernel(XArgs a) {
+__global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq_kernel(XArgs a) {
+  typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
-  constexpr int KT = DQ_KT<M, WR>, WK = NW / WR, NU = KT / 32 / WK;
-  constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
-  constexpr int TILE_BYTES = 2 * KT * DP * (int)sizeof(E);
-  constexpr int JOIN_BYTES = (NW - WR) * DP * 32 * 4;
-  __shared__ __align__(16) char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
+  constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  __shared__ __align__(16) char lds[S::BYTES];
+  __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
   __shared__ uint32_t words[SPAN / 32];
-  E* ks = reinterpret_cast<E*>(lds);
-  E* vs = ks + KT * DP;
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
   const Job j = job_of(a);
@@ -759,55 +864,24 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WR>)) void xattn_dq_kernel
   const float neg = lse == -INFINITY ? -INFINITY : -lse;
   f32x16 acc[DP / 32] = {};
   const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
-  Stage<T, M, DP, KT, 64 * NW> sk, sv;
-  for (int64_t base = k_lo; base < k_hi; base += SPAN) {
-    __syncthreads();
-    span_words(words, keep, base, k_hi, t, 64 * NW);
-    __syncthreads();
-    const int last = (int)min((int64_t)SPAN, k_hi - base);
-    int next = next_tile<KT>(words, 0, last);
-    if (next < last) {
-      sk.load(base + next, k_hi, a.D, k_at, t);
-      sv.load(base + next, k_hi, a.D, v_at, t);
-    }
-    while (next < last) {
-      const int cur = next;
-      __syncthreads();
-      sk.put(ks, words + cur / 32, t);
-      sv.put(vs, words + cur / 32, t);
-      __syncthreads();
-      next = next_tile<KT>(words, cur + KT, last);
-      if (next < last) {
-        sk.load(base + next, k_hi, a.D, k_at, t);
-        sv.load(base + next, k_hi, a.D, v_at, t);
-      }
+  for_tiles<T, M, DP, WR, true>(lds, lds1, words, keep, k_lo, k_hi, a.D, k_at, v_at, t, wave, lane,
+                                [&](const E* ks, const E* vs, const uint32_t* on) {
 #pragma unroll
       for (int u = wk * NU; u < (wk + 1) * NU; ++u) {
-        const uint32_t bits = __builtin_amdgcn_readfirstlane(words[cur / 32 + u]);
+        const uint32_t bits = __builtin_amdgcn_readfirstlane(on[u]);
         if (bits == 0) continue;
         f32x16 s = {}, dp = {};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          s = M::mma(row_frag<M, DP>(ks, 32 * u, c, lane), q[c], s);
-          dp = M::mma(row_frag<M, DP>(vs, 32 * u, c, lane), go[c], dp);
-        }
+        rows_mma2<M, DP>(ks, vs, 32 * u, [&](int c) { return q[c]; }, [&](int c) { return go[c]; },
+                         s, dp, lane);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[r] = exp2_fast(fmaf(s[r], a.c, neg)) * (dp[r] - delta);
         if (bits != ~0u)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[r] = (bits >> acc_row(r, lane)) & 1 ? s[r] : 0.f;
-#pragma unroll
-        for (int c = 0; c < PC; ++c) {
-          const typename M::frag ds = M::pack(s, c);
-#pragma unroll
-          for (int d = 0; d < DP / 32; ++d)
-            acc[d] = M::mma(M::template col<DP>(ks, 32 * u + c * M::CHUNK, 32 * d, lane), ds,
-                            acc[d]);
-        }
+        cols_mma<M, DP>(ks, 32 * u, s, acc, lane);
       }
-    }
-  }
+  });
   if constexpr (WK > 1) {
     __syncthreads();
     float* join = reinterpret_cast<float*>(lds);
@@ -832,22 +906,32 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WR>)) void xattn_dq_kernel
   });
 }
 
-// dK, dV: WC of the block's waves along the keys (32 each), the others along the staged rows, over
-// the rows of every head that shares the keys.
-template <class M, int WC>
-constexpr int DKV_RT = sizeof(typename M::elem) == 2 && WC == NW ? 64 : 32 * (NW / WC);
+// dK, dV: WC of the block's waves along the keys (32 each), the others along the staged rows, RT at a
+// time, over the rows of every head that shares the keys.
+template <class M, int DP, int WC>
+struct DkvShape {
+  typedef typename M::elem E;
+  static constexpr int WS = NW / WC;
+  static constexpr int RT = sizeof(E) == 2 && DP == 64 && WC == NW ? 64 : 32 * WS;
+  static constexpr int NU = RT / 32 / WS;
+  static constexpr int TILE = RT * DP;  // elements of Q, and of dO
+  static constexpr int BUFS = 4 * TILE * (int)sizeof(E) <= 131072 ? 2 : 1;
+  static constexpr int JOIN = (NW - WC) * DP * 32 * 4;  // bytes, at the end: dK, then dV
+  static constexpr int BYTES = 2 * TILE * (int)sizeof(E) > JOIN ? 2 * TILE * (int)sizeof(E) : JOIN;
+  static constexpr bool V_LDS = sizeof(E) == 2 && DP == 128 && WC == NW;
+};
 
 template <class T, class M, int DP, int WC>
-__global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WC>)) void xattn_dkv_kernel(XArgs a) {
+__global__ __launch_bounds__(64 * NW, (Shape<M, DP, WC>::BWD_OCC)) void xattn_dkv_kernel(XArgs a) {
+  typedef DkvShape<M, DP, WC> S;
   typedef typename M::elem E;
-  constexpr int RT = DKV_RT<M, WC>, WS = NW / WC, NU = RT / 32 / WS;
+  constexpr int RT = S::RT, WS = S::WS, NU = S::NU;
   constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
-  constexpr int TILE_BYTES = 2 * RT * DP * (int)sizeof(E);
-  constexpr int JOIN_BYTES = (NW - WC) * DP * 32 * 4;  // dK, then dV
-  __shared__ __align__(16) char lds[TILE_BYTES > JOIN_BYTES ? TILE_BYTES : JOIN_BYTES];
-  __shared__ __align__(16) float st[2][RT];  // -lse (-inf: a row without a key), delta
-  E* qs = reinterpret_cast<E*>(lds);
-  E* gs = qs + RT * DP;
+  __shared__ __align__(16) char lds[S::BYTES];
+  __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
+  // -lse (-inf: a row without a key), then delta, of the tile's rows
+  __shared__ __align__(16) float st0[2 * RT], st1[2 * RT];
+  __shared__ __align__(16) char v_lds[S::V_LDS ? NW * 32 * DP * (int)sizeof(E) : 16];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wc = wave % WC, ws = wave / WC;
   const Job j = job_of(a);
@@ -859,6 +943,16 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WC>)) void xattn_dkv_kerne
                       ok, a.D, lane);
   load_rows<T, M, DP>(v, static_cast<const T*>(a.v) + j.b * a.v_bs + j.hk * a.v_hs + key * a.v_ls,
                       ok, a.D, lane);
+  // V's operand: in registers, or, where those would not do for two waves a SIMD, in the wave's own
+  // part of LDS (read by this wave alone: no barrier)
+  typename M::frag* own = reinterpret_cast<typename M::frag*>(v_lds) + wave * NC * 64 + lane;
+  if constexpr (S::V_LDS)
+#pragma unroll
+    for (int c = 0; c < NC; ++c) own[c * 64] = v[c];
+  const auto v_frag = [&](int c) -> typename M::frag {
+    if constexpr (S::V_LDS) return own[c * 64];
+    else return v[c];
+  };
   const T* q = static_cast<const T*>(a.q) + j.b * a.q_bs;
   const T* go = static_cast<const T*>(a.dout) + j.b * a.do_bs;
   const auto q_at = [&](int64_t r) {
@@ -874,11 +968,11 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WC>)) void xattn_dkv_kerne
   const bool live = __syncthreads_or(ok);  // a tile of padding has no gradient
   const bool mine = __ballot(ok) != 0;
   const bool whole = __ballot(ok) == ~0ull;
-  Stage<T, M, DP, RT, 64 * NW> sq, sg;
   float stat[2] = {-INFINITY, 0.f};
-  const auto load = [&](int r0) {
-    sq.load(r0, r_hi, a.D, q_at, t);
-    sg.load(r0, r_hi, a.D, g_at, t);
+  const auto load = [&](char* to, int r0) {
+    E* qs = reinterpret_cast<E*>(to);
+    stage<E, DP, RT>(qs, r0, r_hi - 1, a.D, q_at, wave, lane);
+    stage<E, DP, RT>(qs + S::TILE, r0, r_hi - 1, a.D, g_at, wave, lane);
     if (t < RT) {
       const bool there = r0 + t < r_hi;
       const RowAt ra = row_at(a, j.hk, there ? r0 + t : 0);
@@ -888,31 +982,27 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WC>)) void xattn_dkv_kerne
       stat[1] = there ? a.delta[at] : 0.f;
     }
   };
-  if (live && r_lo < r_hi) load(r_lo);
-  for (int r0 = r_lo; live && r0 < r_hi; r0 += RT) {
-    __syncthreads();
-    sq.put(qs, nullptr, t);
-    sg.put(gs, nullptr, t);
+  const auto arrive = [&](float* st) {  // what load() began is in LDS for every wave
     if (t < RT) {
-      st[0][t] = stat[0];
-      st[1][t] = stat[1];
+      st[t] = stat[0];
+      st[RT + t] = stat[1];
     }
+    landed();
     __syncthreads();
-    if (r0 + RT < r_hi) load(r0 + RT);
-    if (!mine) continue;
+  };
+  const auto take = [&](const char* from, const float* st) {
+    if (!mine) return;
+    const E* qs = reinterpret_cast<const E*>(from);
+    const E* gs = qs + S::TILE;
 #pragma unroll
     for (int u = ws * NU; u < (ws + 1) * NU; ++u) {
       f32x16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        s = M::mma(row_frag<M, DP>(qs, 32 * u, c, lane), k[c], s);
-        dp = M::mma(row_frag<M, DP>(gs, 32 * u, c, lane), v[c], dp);
-      }
+      rows_mma2<M, DP>(qs, gs, 32 * u, [&](int c) { return k[c]; }, v_frag, s, dp, lane);
 #pragma unroll
       for (int r4 = 0; r4 < 4; ++r4) {
         const int i = 32 * u + acc_row(4 * r4, lane);
-        const f32x4 neg = *reinterpret_cast<const f32x4*>(&st[0][i]);
-        const f32x4 delta = *reinterpret_cast<const f32x4*>(&st[1][i]);
+        const f32x4 neg = *reinterpret_cast<const f32x4*>(&st[i]);
+        const f32x4 delta = *reinterpret_cast<const f32x4*>(&st[RT + i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * r4 + e;
@@ -926,14 +1016,31 @@ __global__ __launch_bounds__(64 * NW, (BWD_OCC<M, DP, WC>)) void xattn_dkv_kerne
           s[r] = ok ? s[r] : 0.f;
           dp[r] = ok ? dp[r] : 0.f;
         }
-#pragma unroll
-      for (int c = 0; c < PC; ++c) {
-        const typename M::frag p = M::pack(s, c), ds = M::pack(dp, c);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) {
-          dv[d] = M::mma(M::template col<DP>(gs, 32 * u + c * M::CHUNK, 32 * d, lane), p, dv[d]);
-          dk[d] = M::mma(M::template col<DP>(qs, 32 * u + c * M::CHUNK, 32 * d, lane), ds, dk[d]);
-        }
+      cols_mma<M, DP>(gs, 32 * u, s, dv, lane);
+      cols_mma<M, DP>(qs, 32 * u, dp, dk, lane);
+    }
+  };
+  if (live && r_lo < r_hi) {
+    load(lds, r_lo);
+    arrive(st0);
+    if constexpr (S::BUFS == 2) {
+      for (int r0 = r_lo;;) {
+        if (r0 + RT < r_hi) load(lds1, r0 + RT);
+        take(lds, st0);
+        if ((r0 += RT) >= r_hi) break;
+        arrive(st1);
+        if (r0 + RT < r_hi) load(lds, r0 + RT);
+        take(lds1, st1);
+        if ((r0 += RT) >= r_hi) break;
+        arrive(st0);
+      }
+    } else {
+      for (int r0 = r_lo + RT;; r0 += RT) {
+        take(lds, st0);
+        if (r0 >= r_hi) break;
+        __syncthreads();
+        load(lds, r0);
+        arrive(st0);
       }
     }
   }
@@ -1115,6 +1222,11 @@ struct MmaOf { typedef MmaF32 type; };
 template <>
 struct MmaOf<bf16> { typedef MmaBf16 type; };
 
+// Tiles go from memory to LDS in 16-byte pieces, which have to lie at multiples of 4 bytes.
+bool pieces_aligned(const void* p, const int64_t* st, int32_t dtype) {
+  return (uintptr_t)p % 4 == 0 && (dtype == MPR_F32 || ((st[0] | st[1] | st[2]) & 1) == 0);
+}
+
 // f(integral constant DP, integral constant NW)
 template <class F>
 int by_tile(int D, int nw, F&& f) {
@@ -1142,12 +1254,12 @@ int few_rows(const XArgs& a, unsigned blocks, hipStream_t s) {
 
 template <class T>
 int xattn_forward(XArgs a, const XPlan& p, hipStream_t s) {
-  typedef typename MmaOf<T>::type M;
   const unsigned blocks = xattn_tile(a, p.fwd);
   if (p.few) {
     MPR_TRY(a.R == 1 ? (few_rows<T, 1>(a, blocks, s)) : a.R == 2 ? (few_rows<T, 2>(a, blocks, s))
             : a.R <= 4 ? (few_rows<T, 4>(a, blocks, s)) : (few_rows<T, 8>(a, blocks, s)));
-  } else {
+  } else if constexpr (!std::is_same_v<T, f16>) {
+    typedef typename MmaOf<T>::type M;
     MPR_TRY(by_tile(a.D, p.fwd.nw, [&](auto dp, auto nw) -> int {
       constexpr int DP = dp, WR = nw;
       xattn_fwd_kernel<T, M, DP, WR><<<blocks, 64 * NW, 0, s>>>(a);
@@ -1231,6 +1343,11 @@ int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* ke
     MPR_REQUIRE(p.fwd_bytes == 0 || (ws && ws_bytes >= p.fwd_bytes),
                 "xattn_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
                 (long long)p.fwd_bytes);
+    MPR_REQUIRE(p.few || dtype != MPR_F16, "xattn_fwd: float16 is for at most %d rows of a key head",
+                FEW_ROWS);
+    MPR_REQUIRE(p.few || dims[4] == 0 || (pieces_aligned(k, strides + 3, dtype) &&
+                                          pieces_aligned(v, strides + 6, dtype)),
+                "xattn_fwd: heads of k or v not at multiples of 4 bytes");
     XArgs a = xattn_args(q, k, v, keep, dims, strides, scale);
     a.out = out;
     a.lse = lse;
@@ -1257,6 +1374,12 @@ int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* ke
     MPR_REQUIRE(p.bwd_bytes == 0 || (ws && ws_bytes >= p.bwd_bytes),
                 "xattn_bwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
                 (long long)p.bwd_bytes);
+    MPR_REQUIRE(dtype != MPR_F16, "xattn_bwd: float16 (compute in float32)");
+    MPR_REQUIRE(dims[3] == 0 || dims[4] == 0 ||
+                    (pieces_aligned(q, strides, dtype) && pieces_aligned(k, strides + 3, dtype) &&
+                     pieces_aligned(v, strides + 6, dtype) &&
+                     pieces_aligned(dout, strides + 10, dtype)),
+                "xattn_bwd: heads not at multiples of 4 bytes");
     XArgs a = xattn_args(q, k, v, keep, dims, strides, scale);
     a.o = out;
     a.lse = const_cast<float*>(lse);
@@ -1267,9 +1390,8 @@ int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* ke
     a.delta = reinterpret_cast<float*>(w + p.delta);
     a.part = reinterpret_cast<float*>(w + up256((int64_t)a.B * a.H * a.Lq * 4));
     a.part2 = reinterpret_cast<float*>(w + p.part2);
-    return by_dtype(dtype, [&](auto z) -> int {
-      return xattn_backward<decltype(z)>(a, p, op_stream(stream));
-    });
+    return dtype == MPR_F32 ? xattn_backward<float>(a, p, op_stream(stream))
+                            : xattn_backward<bf16>(a, p, op_stream(stream));
   });
 }
 

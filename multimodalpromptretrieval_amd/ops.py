@@ -195,6 +195,18 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
 
 
 # ---- cross attention -----------------------------------------------------------------------------
+_FEW_ROWS = 8  # rows of a key head that the single-token kernel takes, in any type
+
+
+def _heads(t):
+    """The tensor with the elements of a head adjacent and every head at a multiple of 4 bytes."""
+    b, l, h, d = t.stride()
+    if d == 1 and (t.dtype == torch.float32 or
+                   not ((b | l | h) & 1 or t.data_ptr() & 3)):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t.clone()
+
+
 def _xattn_dims(q, k):
     B, Lq, H, D = q.shape
     return B, H, k.shape[2], Lq, k.shape[1], D
@@ -231,7 +243,7 @@ def _xattn_fwd(q, k, v, keep, scale, want_lse):
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, keep, scale):
-        q, k, v = _rows(q), _rows(k), _rows(v)
+        q, k, v = _heads(q), _heads(k), _heads(v)
         out, lse = _xattn_fwd(q, k, v, keep, scale, True)
         ctx.save_for_backward(q, k, v, keep, out, lse)
         ctx.scale = scale
@@ -241,7 +253,7 @@ class _CrossAttention(torch.autograd.Function):
     @_first_order
     def backward(ctx, dout):
         q, k, v, keep, out, lse = ctx.saved_tensors
-        dout = _rows(dout)
+        dout = _heads(dout)
         code, dims = _DTYPES[q.dtype], _xattn_dims(q, k)
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
 
@@ -267,7 +279,9 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
     ``key_mask`` [B, Lk] (or [1, Lk]): the keys that are not 0 / False are attended to; what a
     masked key holds (NaN, infinities) touches nothing and its gradient is 0, and a row whose keys
     are all masked, or Lk = 0, gives 0.  Any strides will do (the halves of a joint k | v
-    projection), but the elements of a head are read in place only if they are adjacent."""
+    projection); heads are read in place where their elements are adjacent and they begin at
+    multiples of 4 bytes, and copied otherwise.  float16 is computed in float32 except for single
+    tokens (up to 8 rows of queries to a key head, without gradients)."""
     _floating(q, "cross_attention q")
     for t, name in ((k, "k"), (v, "v")):
         _floating(t, "cross_attention " + name)
@@ -297,12 +311,15 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
     _on_gpu(q, "cross_attention")
     if scale < 0.0:  # the kernels' running maximum is of unscaled scores
         q, scale = -q, -scale
+    grad = (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled()
+    if q.dtype == torch.float16 and (grad or H // Hkv * q.shape[1] > _FEW_ROWS):
+        return cross_attention(q.float(), k.float(), v.float(), key_mask, scale).to(q.dtype)
     if key_mask is not None:
         keep = key_mask if key_mask.dtype == torch.bool else key_mask != 0
         keep = _rows(keep.detach().expand(B, Lk)).view(torch.uint8)
-    if (q.requires_grad or k.requires_grad or v.requires_grad) and torch.is_grad_enabled():
+    if grad:
         return _CrossAttention.apply(q, k, v, keep, scale)
-    return _xattn_fwd(_rows(q), _rows(k), _rows(v), keep, scale, False)[0]
+    return _xattn_fwd(_heads(q), _heads(k), _heads(v), keep, scale, False)[0]
 
 
 # ---- log-probabilities and the preference loss -----------------------------------------------------
