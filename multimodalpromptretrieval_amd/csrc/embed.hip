@@ -10,6 +10,7 @@
 // An id outside [0, V) reads nothing: its output row is NaN, and it has no gradient.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops.h"
 
@@ -19,7 +20,7 @@ namespace {
 // ---- lookup --------------------------------------------------------------------------------------
 constexpr int LOOKUP_ROWS = 4;  // rows a wave has in flight
 
-template <class T, class I>
+template <class T, class I, bool STREAM>
 __global__ __launch_bounds__(256) void embed_lookup_kernel(const T* __restrict__ table, int64_t V,
                                                            int64_t ld, const I* __restrict__ ids,
                                                            int64_t n, int d, float scale,
@@ -49,7 +50,7 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const T* __restrict__
     }
 #pragma unroll
     for (int r = 0; r < LOOKUP_ROWS; ++r)
-      if (r0 + r < n) store_f<T, N>(out + (r0 + r) * d + (int64_t)c * N, x[r]);
+      if (r0 + r < n) store_f<T, N, STREAM>(out + (r0 + r) * d + (int64_t)c * N, x[r]);
   }
   for (int c = nv * N + lane; c < d; c += 64)
     for (int r = 0; r < LOOKUP_ROWS; ++r)
@@ -65,7 +66,7 @@ __global__ __launch_bounds__(256) void embed_lookup_kernel(const T* __restrict__
 // no gradient (the padding index, ids outside the table) become V and sort behind every row.
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WAVES = SORT_THREADS / 64;
-constexpr int SORT_ITEMS = 4;  // per thread
+constexpr int SORT_ITEMS = 2;  // per thread
 constexpr int SORT_TILE = SORT_THREADS * SORT_ITEMS;
 constexpr int SORT_BLOCKS = 256;
 constexpr int SORT_ONE = 16 * SORT_THREADS;  // positions that one launch sorts
@@ -164,7 +165,7 @@ __device__ __forceinline__ uint32_t digit_rank(uint32_t* cnt, uint32_t dig, bool
 // range) by itself.  It reads every id, counts those below its range (which says where its part of
 // the result begins) and keeps its own in the order of their positions; one counting pass over
 // `range` digits then ranks them.  Reading 16384 ids in 128 blocks costs less than the launches
-// that sharing them would take: 8992 ids 9 us against 28 us for the two passes above.
+// that sharing them would take: 8992 ids 13 us against 28 us for the two passes below.
 constexpr int RANGE_MAX = 1024;
 template <int ITEMS>
 __global__ __launch_bounds__(SORT_THREADS) void sort_range_kernel(KeySrc src, int n, uint32_t range,
@@ -260,12 +261,21 @@ __global__ __launch_bounds__(SORT_THREADS) void sort_move_kernel(KeySrc src, int
   __shared__ uint32_t wcnt[SORT_WAVES][DIGITS];    // per wave: items of the digit, then their base
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   const uint32_t mask = (1u << bits) - 1;
+  // each digit's items in the blocks before this one, and in all (four threads a digit)
   uint32_t before = 0, total = 0;
+#pragma unroll 8
+  for (int b = t / DIGITS; b < (int)gridDim.x; b += SORT_THREADS / DIGITS) {
+    const uint32_t h = hist[(int64_t)b * DIGITS + t % DIGITS];
+    if (b < (int)blockIdx.x) before += h;
+    total += h;
+  }
+  (&wcnt[0][0])[2 * t] = before;
+  (&wcnt[0][0])[2 * t + 1] = total;
+  __syncthreads();
   if (t < DIGITS)
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-      const uint32_t h = hist[(int64_t)b * DIGITS + t];
-      if (b < (int)blockIdx.x) before += h;
-      total += h;
+    for (int q = 1; q < SORT_THREADS / DIGITS; ++q) {
+      before += (&wcnt[0][0])[2 * (t + q * DIGITS)];
+      total += (&wcnt[0][0])[2 * (t + q * DIGITS) + 1];
     }
   const uint32_t smaller = scan_digits(total, part);
   if (t < DIGITS) base[t] = smaller + before;
@@ -410,13 +420,13 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
 }
 
 // A run that crosses windows: the tail of the window where it begins, then the heads of the
-// following ones.  A block per window and 64 columns; the waves take the windows in turn.
+// following ones.  A block per window and 256 columns (4 a lane); the waves take the windows in turn.
 constexpr int JOIN_AHEAD = 8;
-template <class T>
+template <class T, int N>
 __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, T* __restrict__ dw) {
-  __shared__ float red[4][64];
+  __shared__ float red[4][64][N];
   const int64_t w = blockIdx.x;
-  const int64_t hi = min(a.n, (w + 1) * a.win);
+  const int64_t hi = (w + 1) * a.win;
   if (hi >= a.n) return;
   const uint32_t key = a.key[hi - 1];
   if (key >= (uint32_t)a.V || a.key[hi] != key) return;
@@ -435,26 +445,37 @@ __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, T* __restric
     m += __ffsll((unsigned long long)~same) - 1;
     break;
   }
-  const int col = blockIdx.y * 64 + lane;
-  float s = 0.f;
+  const int col = (blockIdx.y * 64 + lane) * N;
+  float s[N] = {};
   if (col < a.d) {
     const float* h = a.head + (w + 1) * a.d + col;
     int64_t i = wave;
     for (; i + 4 * (JOIN_AHEAD - 1) < m; i += 4 * JOIN_AHEAD) {
-      float x[JOIN_AHEAD];
+      float x[JOIN_AHEAD][N];
 #pragma unroll
-      for (int j = 0; j < JOIN_AHEAD; ++j) x[j] = h[(i + 4 * j) * a.d];
+      for (int j = 0; j < JOIN_AHEAD; ++j) load_f<float, N>(h + (i + 4 * j) * a.d, x[j]);
 #pragma unroll
-      for (int j = 0; j < JOIN_AHEAD; ++j) s += x[j];
+      for (int j = 0; j < JOIN_AHEAD; ++j)
+#pragma unroll
+        for (int e = 0; e < N; ++e) s[e] += x[j][e];
     }
-    for (; i < m; i += 4) s += h[i * a.d];
+    for (; i < m; i += 4) {
+      float x[N];
+      load_f<float, N>(h + i * a.d, x);
+#pragma unroll
+      for (int e = 0; e < N; ++e) s[e] += x[e];
+    }
   }
-  red[wave][lane] = s;
+#pragma unroll
+  for (int e = 0; e < N; ++e) red[wave][lane][e] = s[e];
   __syncthreads();
   if (wave == 0 && col < a.d) {
-    const float v = a.tail[w * a.d + col] + ((red[0][lane] + red[1][lane]) +
-                                             (red[2][lane] + red[3][lane]));
-    dw[(int64_t)key * a.d + col] = from_f<T>(v * a.scale);
+    load_f<float, N>(a.tail + w * a.d + col, s);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      s[e] = (s[e] + ((red[0][lane][e] + red[1][lane][e]) + (red[2][lane][e] + red[3][lane][e]))) *
+             a.scale;
+    store_f<T, N>(dw + (int64_t)key * a.d + col, s);
   }
 }
 
@@ -468,16 +489,16 @@ struct EmbedGrad {
 
 int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// Window: the largest of 256 / 64 / 16 / 8 positions that still gives SUM_WAVES waves (a longer
-// window leaves fewer partial sums of the runs that cross windows; fewer waves leave memory idle).
-constexpr int64_t SUM_WAVES = 2048;
+// Window: the largest of 256 .. 8 positions that still gives SUM_WAVES waves (a longer window leaves
+// fewer partial sums of the runs that cross windows; fewer waves leave memory idle).
+constexpr int64_t SUM_WAVES = 4096;
 
 EmbedGrad embed_plan(int64_t n, int64_t V, int d, int vec) {
   EmbedGrad p;
   p.sort = sort_plan(n, V);
   p.slabs = (int)cdiv(d, 64 * (int64_t)vec);
   p.win = 8;
-  for (int w : {256, 64, 16})
+  for (int w : {256, 128, 64, 32, 16})
     if (n / w * p.slabs >= SUM_WAVES) {
       p.win = w;
       break;
@@ -507,7 +528,8 @@ int embed_sums(const void* dout, const SumArgs& a, void* dw, hipStream_t s) {
   embed_sum_kernel<T, N><<<dim3((unsigned)blocks), 256, 0, s>>>(static_cast<const T*>(dout), a,
                                                                  static_cast<T*>(dw));
   MPR_LAUNCHED();
-  embed_join_kernel<T><<<dim3((unsigned)a.wins, (unsigned)cdiv(a.d, 64)), 256, 0, s>>>(
+  constexpr int J = N == 1 ? 1 : 4;  // (N > 1: d is a multiple of it)
+  embed_join_kernel<T, J><<<dim3((unsigned)a.wins, (unsigned)cdiv(a.d, 64 * J)), 256, 0, s>>>(
       a, static_cast<T*>(dw));
   MPR_LAUNCHED();
   return MPR_OK;
@@ -538,14 +560,17 @@ int mpr_embed_lookup(const void* table, int32_t dtype, int64_t V, int64_t ld, co
     return by_dtype(dtype, [&](auto z) -> int {
       using T = decltype(z);
       const dim3 grid((unsigned)cdiv(n, 4 * LOOKUP_ROWS));
-      if (ids64)
-        embed_lookup_kernel<T, int64_t><<<grid, 256, 0, op_stream(stream)>>>(
-            static_cast<const T*>(table), V, ld, static_cast<const int64_t*>(ids), n, d, scale,
+      const bool stream_out = n * d * (int64_t)sizeof(T) >= STREAM_BYTES;
+      const auto launch = [&](auto id, auto st) {
+        typedef decltype(id) I;
+        embed_lookup_kernel<T, I, decltype(st)::value><<<grid, 256, 0, op_stream(stream)>>>(
+            static_cast<const T*>(table), V, ld, static_cast<const I*>(ids), n, d, scale,
             static_cast<T*>(out));
-      else
-        embed_lookup_kernel<T, int32_t><<<grid, 256, 0, op_stream(stream)>>>(
-            static_cast<const T*>(table), V, ld, static_cast<const int32_t*>(ids), n, d, scale,
-            static_cast<T*>(out));
+      };
+      if (ids64 && stream_out) launch(int64_t{}, std::true_type{});
+      else if (ids64) launch(int64_t{}, std::false_type{});
+      else if (stream_out) launch(int32_t{}, std::true_type{});
+      else launch(int32_t{}, std::false_type{});
       MPR_LAUNCHED();
       return MPR_OK;
     });

@@ -49,6 +49,24 @@ __device__ __forceinline__ void store_f(T* p, const float (&x)[N]) {
   *reinterpret_cast<typename Vec<T, N>::type*>(p) = v;
 }
 
+// STREAM: past the caches, for results larger than they are.  Written the usual way, such a result
+// leaves the 256 MB Infinity Cache full of lines that the next kernels' reads have to wait out:
+// 262144 looked-up rows of 2 KB and the gradient after them 310 us, streamed 283.
+template <class T, int N, bool STREAM>
+__device__ __forceinline__ void store_f(T* p, const float (&x)[N]) {
+  if constexpr (STREAM) {
+    typename Vec<T, N>::type v;
+    if constexpr (N == 1) v = from_f<T>(x[0]);
+    else
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = from_f<T>(x[i]);
+    __builtin_nontemporal_store(v, reinterpret_cast<typename Vec<T, N>::type*>(p));
+  } else {
+    store_f<T, N>(p, x);
+  }
+}
+constexpr int64_t STREAM_BYTES = (int64_t)256 << 20;
+
 template <class A>
 __device__ __forceinline__ A wave_add(A v) {
 #pragma unroll

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(1024) void lp_few_kernel(const T* x, LpArgs a, cons
   lp_pairs(lp64, ref, a.S / 2, beta, eps, loss, dlp);
 }
 
-template <class T>
+template <class T, bool STREAM>
 __global__ __launch_bounds__(LP_THREADS) void lp_grad_kernel(const T* __restrict__ x, LpArgs a,
                                                              const MaxSum* __restrict__ row_stat,
                                                              const float* __restrict__ dlp,
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(LP_THREADS) void lp_grad_kernel(const T* __restrict
   const bool rest = blockIdx.y == gridDim.y - 1;
   if (y < 0) {
     const float z[N] = {};
-    for (int64_t i = lo + threadIdx.x; i < hi; i += LP_THREADS) store_f<T, N>(dr + i * N, z);
+    for (int64_t i = lo + threadIdx.x; i < hi; i += LP_THREADS) store_f<T, N, STREAM>(dr + i * N, z);
     if (rest)
       for (int64_t j = nv * N + threadIdx.x; j < a.V; j += LP_THREADS) dr[j] = from_f<T>(0.f);
     return;
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(LP_THREADS) void lp_grad_kernel(const T* __restrict
     if (at >= 0 && at < N)
 #pragma unroll
       for (int e = 0; e < N; ++e) v[e] += e == at ? g : 0.f;
-    store_f<T, N>(dr + i * N, v);
+    store_f<T, N, STREAM>(dr + i * N, v);
   }
   if (rest)
     for (int64_t j = nv * N + threadIdx.x; j < a.V; j += LP_THREADS)
@@ -326,7 +326,9 @@ int mpr_logps_bwd(const void* logits, int32_t dtype, int64_t S, int64_t T, int64
     const LpArgs a{labels, labels64, ls, xs, xt, S, T, V, p.split};
     return by_dtype(dtype, [&](auto z) -> int {
       using X = decltype(z);
-      lp_grad_kernel<X><<<dim3((unsigned)p.rows, p.split), LP_THREADS, 0, op_stream(stream)>>>(
+      const auto grad = p.rows * V * (int64_t)sizeof(X) >= STREAM_BYTES ? lp_grad_kernel<X, true>
+                                                                          : lp_grad_kernel<X, false>;
+      grad<<<dim3((unsigned)p.rows, p.split), LP_THREADS, 0, op_stream(stream)>>>(
           static_cast<const X*>(logits), a, reinterpret_cast<const MaxSum*>(row_stat), dlogps,
           mult, static_cast<X*>(dlogits));
       MPR_LAUNCHED();

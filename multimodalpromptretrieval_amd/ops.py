@@ -33,6 +33,7 @@ import ctypes
 import math
 from array import array
 from functools import lru_cache
+from operator import attrgetter
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -455,57 +456,73 @@ def _dense(t) -> bool:
     return True
 
 
-def _codes(tensors, what):
-    try:  # hundreds of tensors a call: the names of what is wrong are made only then
-        return [_DTYPES[t.dtype] for t in tensors]
-    except (KeyError, AttributeError):
-        return [_floating(t, f"{what} {i}") for i, t in enumerate(tensors)]
+_T = torch.Tensor
+_dtype_of = attrgetter("dtype")
+
+
+def _plain(tensors):
+    """(dtype codes, device index) of contiguous tensors of the known types on one device, else None.
+    A model has hundreds of gradients, so each question goes to all of them in one C loop; what the
+    answer None hides is found out and named by the functions below."""
+    try:
+        codes = list(map(_DTYPES.get, map(_dtype_of, tensors)))
+        devices = set(map(_T.get_device, tensors))
+        if None in codes or len(devices) != 1 or not all(map(_T.is_contiguous, tensors)):
+            return None
+    except (TypeError, AttributeError, RuntimeError):
+        return None
+    return codes, devices.pop()
 
 
 def _check_grads(grads, what):
-    """(device, dtype codes) of the gradients, or the refusal of the first that will not do."""
-    codes = _codes(grads, what + " gradient")
-    device, index = grads[0].device, grads[0].get_device()
+    """The dtype codes of the gradients, or the refusal of the first that will not do."""
+    codes = [_floating(g, f"{what} gradient {i}") for i, g in enumerate(grads)]
+    device = grads[0].device
     for i, g in enumerate(grads):
-        if g.get_device() != index or g.layout is not torch.strided:
+        if g.device != device or g.layout is not torch.strided:
             raise ValueError(f"{what}: gradient {i} is a {g.layout} tensor on {g.device}, needed "
                              f"dense on {device}")
         if not (g.is_contiguous() or _dense(g)):
             raise ValueError(f"{what}: gradient {i} {tuple(g.shape)} with strides {g.stride()} "
                              "leaves gaps in its memory (clip a .contiguous() copy)")
-    return device, codes
+    return codes
 
 
-def _check_outs(grads, out, device, what):
-    if len(out) != len(grads):
-        raise ValueError(f"{what}: {len(grads)} gradients and {len(out)} outputs")
-    codes = _codes(out, what + " output")
-    index = grads[0].get_device()
+def _check_outs(grads, out, what):
+    codes = [_floating(t, f"{what} output {i}") for i, t in enumerate(out)]
     for i, (g, t) in enumerate(zip(grads, out)):
-        if t.get_device() != index or t.shape != g.shape:
+        dense = t.is_contiguous() and g.is_contiguous()
+        if t.device != g.device or t.numel() != g.numel() or not (dense or t.shape == g.shape):
             raise ValueError(f"{what}: output {i} is {tuple(t.shape)} on {t.device}, its gradient "
-                             f"{tuple(g.shape)} on {device}")
-        if not (t.is_contiguous() and g.is_contiguous()) and t.stride() != g.stride():
+                             f"{tuple(g.shape)} on {g.device}")
+        if not dense and t.stride() != g.stride():
             raise ValueError(f"{what}: output {i} is laid out otherwise than its gradient")
     return codes
 
 
 def _clip(grads, out, max_norm, eps, what):
     n = len(grads)
+    if out is not None and len(out) != n:
+        raise ValueError(f"{what}: {n} gradients and {len(out)} outputs")
     if n == 0:
-        if out:
-            raise ValueError(f"{what}: 0 gradients and {len(out)} outputs")
         return torch.zeros(())
-    device, codes = _check_grads(grads, what)
-    into = codes if out is None else _check_outs(grads, out, device, what)
+    mine = _plain(grads)
+    codes = mine[0] if mine else _check_grads(grads, what)
+    counts = array("q", map(_T.numel, grads))
+    if out is not None:
+        theirs = _plain(out)
+        if not (mine and theirs and theirs[1] == mine[1] and
+                counts == array("q", map(_T.numel, out))):
+            theirs = (_check_outs(grads, out, what),)
     _on_gpu(grads[0], what)
+    device = grads[0].device
     table = array("q", bytes(40 * n))  # n x {pointer, values, type, output pointer, its type}
-    table[0::5] = array("q", [g.data_ptr() for g in grads])
-    table[1::5] = array("q", [g.numel() for g in grads])
+    table[0::5] = array("q", map(_T.data_ptr, grads))
+    table[1::5] = counts
     table[2::5] = array("q", codes)
     if max_norm is not None:
-        table[3::5] = table[0::5] if out is None else array("q", [t.data_ptr() for t in out])
-        table[4::5] = array("q", into)
+        table[3::5] = table[0::5] if out is None else array("q", map(_T.data_ptr, out))
+        table[4::5] = array("q", codes if out is None else theirs[0])
     desc = (ctypes.c_int64 * (5 * n)).from_buffer(table)
     norm = torch.empty((), dtype=torch.float32, device=device)
     nbytes = ctypes.c_int64()
@@ -528,8 +545,8 @@ def clip_grads_(grads, max_norm: float, eps: float = 1e-6, out=None):
     """Scales the gradients by ``min(1, max_norm / (norm + eps))`` and returns ``norm``, their
     global L2 norm before it (``grad_norm``).
 
-    In place, or into ``out``: a tensor for each gradient, of its shape and any floating type (the
-    optimizer's fp32 buffer for bf16 gradients).  Gradients below the limit are not written in
+    In place, or into ``out``: a tensor for each gradient, of its shape (or, both contiguous, its
+    number of values) and any floating type (the optimizer's fp32 buffer for bf16 gradients).  Gradients below the limit are not written in
     place at all.  The types may differ between tensors.  A norm that is not finite goes through as
     it is: NaN makes every gradient NaN, infinity makes finite ones 0.  Tensors that share memory
     (one gradient listed twice) and gradients with gaps in their memory are refused."""
