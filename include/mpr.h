@@ -431,8 +431,8 @@ int mpr_embed_bwd(const float* dY, int32_t d, const int32_t* uniq, const int32_t
  *   Hkv, D a multiple of 8 up to 128, elements of a head contiguous; keep [B, Lk] bytes (0: the key
  *   counts for nothing, whatever it holds) or NULL.  scale >= 0.  dims = {B, H, Hkv, Lq, Lk, D}; strides (in
  *   elements) = {q batch, position, head, k .., v .., keep batch, dout batch, position, head (bwd
- *   only)}.  out [B, Lq, H, D], lse [B, H, Lq] (base-2 log of the rows' sums; may be NULL in a
- *   forward alone), dq as out (NULL: not wanted), dk / dv [B, Lk, Hkv, D] (both or none), all
+ *   only)}.  out [B, Lq, H, D], rest as out (bfloat16: what rounding took off out; NULL: not kept),
+ *   lse [B, H, Lq] (base-2 log of the rows' sums); rest and lse may be NULL in a forward alone; dq as out (NULL: not wanted), dk / dv [B, Lk, Hkv, D] (both or none), all
  *   contiguous.  Heads lie at multiples of 4 bytes.  float16: forward, H / Hkv Lq <= 8 only.  A row without a key: 0.
  *   mpr_logps_fwd: logps[s] = sum over t with labels[s, t] >= 0 of log softmax(logits[s, t])[label]
  *   (logits [S, T, V] with strides xs, xt, 1; labels row stride ls; a label >= V gives NaN), and
@@ -454,11 +454,11 @@ int mpr_embed_grad(const void* dout, int32_t dtype, int64_t ld, const void* ids,
 int mpr_xattn_workspace(const int64_t* dims, int32_t dtype, int64_t* fwd_bytes,
                         int64_t* bwd_bytes);
 int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
-                  const int64_t* dims, const int64_t* strides, float scale, void* out, float* lse,
-                  void* ws, int64_t ws_bytes, void* stream);
+                  const int64_t* dims, const int64_t* strides, float scale, void* out, void* rest,
+                  float* lse, void* ws, int64_t ws_bytes, void* stream);
 int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
                   const int64_t* dims, const int64_t* strides, float scale, const void* out,
-                  const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                  const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
                   int64_t ws_bytes, void* stream);
 int mpr_logps_workspace(int64_t S, int64_t T, int64_t V, int64_t* bytes);
 int mpr_logps_fwd(const void* logits, int32_t dtype, int64_t S, int64_t T, int64_t V, int64_t xs,

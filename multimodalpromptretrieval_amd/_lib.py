@@ -166,10 +166,11 @@ SIGNATURES = [
                                  c_void_p]),
     ("mpr_xattn_workspace", c_int32, [I64P, c_int32, I64P, I64P]),
     ("mpr_xattn_fwd", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, I64P, I64P,
-                                c_float, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+                                c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                c_void_p]),
     ("mpr_xattn_bwd", c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, I64P, I64P,
                                 c_float, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
-                                c_void_p, c_void_p, c_int64, c_void_p]),
+                                c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     ("mpr_logps_workspace", c_int32, [c_int64, c_int64, c_int64, I64P]),
     ("mpr_logps_fwd", c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64,
                                 c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p,

@@ -13,8 +13,10 @@
 // leave half's range, so the caller computes them in float.  The products are arranged so that a tile's scores come out of the matrix core in the
 // lane order in which the next product takes them (scores transposed: lane = row, registers =
 // keys): probabilities go from one product to the next in registers, never through LDS.  P and dS
-// are rounded to bf16 as operands of the second products (half a step, 2^-9 relative each), as the
-// inputs are; sums stay fp32.
+// are rounded to bf16 as operands of the second products, as the inputs are; sums stay fp32.  Two
+// things keep the backward's differences dP - rowsum(dO O) exact where a row has few keys and they
+// cancel: the forward divides by the sum of the rounded P (its weights then add up to 1), and it
+// keeps what rounding takes off O for that row sum.
 //
 // Masked keys count for nothing whatever they hold (NaN, infinities): they are staged as zeros.
 #include <algorithm>
@@ -48,6 +50,8 @@ struct XArgs {
   float slack;       // how far scores may pass the running maximum: 8 / c
   float scale;
   void* out;         // forward: [B, Lq, H, D]
+  void* rest;        // bf16 only, may be null: what rounding took off out
+  const void* o_rest;
   float* lse;        // [B, H, Lq]: max + log2(sum) of the scaled scores in base 2
   float* delta;      // [B, H, Lq]
   float *part, *part2;  // splits' shares
@@ -92,6 +96,14 @@ struct MmaBf16 {
     for (int j = 0; j < 8; ++j) f[j] = (bf16)x[8 * c + j];
     return f;
   }
+  static __device__ __forceinline__ float sum(frag f, float s) {  // s + its elements
+    typedef bf16 pair __attribute__((ext_vector_type(2)));
+    const pair one = {(bf16)1.f, (bf16)1.f};
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+      s = __builtin_amdgcn_fdot2_f32_bf16(pair{f[j], f[j + 1]}, one, s, false);
+    return s;
+  }
   static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
@@ -112,6 +124,9 @@ struct MmaF32 {
   }
   static __device__ __forceinline__ frag pack(const f32x16& x, int c) {
     return frag{x[4 * c], x[4 * c + 1], x[4 * c + 2], x[4 * c + 3]};
+  }
+  static __device__ __forceinline__ float sum(frag f, float s) {
+    return s + ((f[0] + f[1]) + (f[2] + f[3]));
   }
   static __device__ __forceinline__ f32x16 mma(frag a, frag b, f32x16 c) {
 #pragma unroll
@@ -181,26 +196,40 @@ __device__ __forceinline__ void rows_mma2(const typename M::elem* p1, const type
     in_order();
   }
 }
-// acc[d] += (columns 32 d .. of LDS rows k0 .. k0 + 31, transposed) x s, s a result of 32 x 32
-template <class M, int DP>
-__device__ __forceinline__ void cols_mma(const typename M::elem* p, int k0, const f32x16& s,
-                                         f32x16 (&acc)[DP / 32], int lane) {
+// acc[d] += (columns 32 d .. of LDS rows k0 .. k0 + 31, transposed) x s, s a result of 32 x 32; the
+// sum of this lane's s, as the product takes them (rounded).  FINE: s in two parts, its rounding and
+// what that takes off it, each multiplied: s to 16 bits instead of 8.
+template <class M, int DP, bool FINE = false>
+__device__ __forceinline__ float cols_mma(const typename M::elem* p, int k0, const f32x16& s,
+                                          f32x16 (&acc)[DP / 32], int lane) {
   constexpr int ND = DP / 32, PC = 32 / M::CHUNK, NI = ND * PC, A = AHEAD < NI ? AHEAD : NI;
-  typename M::frag x[A], f[PC];
+  typename M::frag x[A], f[PC], g[FINE ? PC : 1];
   const auto get = [&](int i) {
     return M::template col<DP>(p, k0 + i / ND * M::CHUNK, i % ND * 32, lane);
   };
 #pragma unroll
   for (int i = 0; i < A; ++i) x[i] = get(i);
+  float sum = 0.f;
 #pragma unroll
-  for (int c = 0; c < PC; ++c) f[c] = M::pack(s, c);
+  for (int c = 0; c < PC; ++c) {
+    f[c] = M::pack(s, c);
+    sum = M::sum(f[c], sum);
+    if constexpr (FINE) {
+      constexpr int N = M::CHUNK / 2;
+#pragma unroll
+      for (int j = 0; j < N; ++j) g[c][j] = (typename M::elem)(s[N * c + j] - (float)f[c][j]);
+      sum = M::sum(g[c], sum);
+    }
+  }
   in_order();
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
     acc[i % ND] = M::mma(x[i % A], f[i / ND], acc[i % ND]);
+    if constexpr (FINE) acc[i % ND] = M::mma(x[i % A], g[i / ND], acc[i % ND]);
     if (i + A < NI) x[i % A] = get(i + A);
     in_order();
   }
+  return sum;
 }
 
 // the row (0 .. 31) that result register r of this lane's half holds
@@ -331,6 +360,18 @@ __device__ __forceinline__ void acc_join(const float* lds, f32x16 (&acc)[NT], fl
     }
 }
 
+// N values of the output, and what rounding takes off them
+template <class T, int N>
+__device__ __forceinline__ void store_out(const XArgs& a, int64_t at, const float (&x)[N]) {
+  store_f<T, N>(static_cast<T*>(a.out) + at, x);
+  if (a.rest) {
+    float y[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) y[e] = x[e] - to_f<T>(from_f<T>(x[e]));
+    store_f<T, N>(static_cast<T*>(a.rest) + at, y);
+  }
+}
+
 struct RowAt {  // row r of (b, key head): its query head and position
   int h, i;
 };
@@ -368,7 +409,7 @@ struct Shape {
   static constexpr int WK = NW / WR;
   static constexpr int KT = HALF && WR == NW ? 64 : 32 * WK;
   static constexpr int NU = KT / 32 / WK;  // a wave's 32-key products in a tile
-  static constexpr int FWD_OCC = HALF ? (DP == 64 ? 3 : 2) : (DP == 64 ? 2 : 1);
+  static constexpr int FWD_OCC = HALF && DP == 64 ? 3 : 2;
   static constexpr int BWD_OCC = HALF || (DP == 64 && WR == NW) ? 2 : 1;
   static constexpr int TILE = KT * DP;  // elements of K, and of V
   static constexpr int BUFS = 4 * TILE * (int)sizeof(E) <= 131072 ? 2 : 1;
@@ -445,7 +486,8 @@ __device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* word
 // ---- forward -------------------------------------------------------------------------------------
 // The running maximum follows the scores only when they pass it by more than 8 (in base 2): until
 // then exponentials up to 2^8 share the old base, and the sums need no rescaling.
-template <class T, class M, int DP, int WR>
+// FINE: P to 16 bits as an operand (bf16).
+template <class T, class M, int DP, int WR, bool FINE>
 __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fwd_kernel(XArgs a) {
   typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
@@ -508,17 +550,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
         for (int d = 0; d < DP / 32; ++d) acc[d] *= alpha;
       }
       const float zero = m == -INFINITY ? 0.f : -m * a.c;
-      float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int u = 0; u < NU; ++u)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[u][r] = exp2_fast(fmaf(s[u][r], a.c, zero));
-          sum[r & 1] += s[u][r];
-        }
-      l += sum[0] + sum[1];
+        for (int r = 0; r < 16; ++r) s[u][r] = exp2_fast(fmaf(s[u][r], a.c, zero));
 #pragma unroll
-      for (int u = 0; u < NU; ++u) cols_mma<M, DP>(vs, 32 * (u0 + u), s[u], acc, lane);
+      for (int u = 0; u < NU; ++u) l += cols_mma<M, DP, FINE>(vs, 32 * (u0 + u), s[u], acc, lane);
   });
   l = halves(l, [](float x, float y) { return x + y; });
   if constexpr (WK > 1) {  // the waves along the keys
@@ -557,10 +594,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* o = static_cast<T*>(a.out) + (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+  const int64_t at = (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) * a.D;
   for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
     const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
-    if (d < a.D) store_f<T, 4>(o + d, y);
+    if (d < a.D) store_out<T, 4>(a, at + d, y);
   });
   if (lane < 32 && a.lse)
     a.lse[((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m * a.c + log2f(l);
@@ -591,11 +628,12 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
   const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
   const RowAt ra = row_at(a, hk, (int)(at % a.R));
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(a.out) + (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
+  const int64_t to = (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int d = lane + 64 * j;
-    if (d < a.D) out[d] = from_f<T>(o[j] * inv);
+    const float y[1] = {o[j] * inv};
+    if (d < a.D) store_out<T, 1>(a, to + d, y);
   }
   if (lane == 0 && a.lse)
     a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m + log2f(l);
@@ -784,8 +822,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
       }
     } else {
       const RowAt ra = row_at(a, hk, r);
-      static_cast<T*>(a.out)[(((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D + d] =
-          from_f<T>(sum == 0.f ? 0.f : x / sum);
+      const float y[1] = {sum == 0.f ? 0.f : x / sum};
+      store_out<T, 1>(a, (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D + d, y);
       if (d == 0 && a.lse)
         a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] =
             sum == 0.f ? -INFINITY : top + log2f(sum);
@@ -806,13 +844,14 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
   const int h = (int)(row % a.H);
   const int64_t bi = row / a.H;
   const int i = (int)(bi % a.Lq), b = (int)(bi / a.Lq);
-  for (int d = N * half; in && d < a.D; d += M::CHUNK) {
-    float x[N], y[N];
-    load_f<T, N>(static_cast<const T*>(a.o) + row * a.D + d, x);
-    load_f<T, N>(static_cast<const T*>(a.dout) + b * a.do_bs + i * a.do_ls + h * a.do_hs + d, y);
+  for (const void* part : {a.o, a.o_rest})
+    for (int d = N * half; part && in && d < a.D; d += M::CHUNK) {
+      float x[N], y[N];
+      load_f<T, N>(static_cast<const T*>(part) + row * a.D + d, x);
+      load_f<T, N>(static_cast<const T*>(a.dout) + b * a.do_bs + i * a.do_ls + h * a.do_hs + d, y);
 #pragma unroll
-    for (int e = 0; e < N; ++e) s = fmaf(y[e], x[e], s);
-  }
+      for (int e = 0; e < N; ++e) s = fmaf(y[e], x[e], s);
+    }
   s += __shfl_xor(s, 1, 64);
   if (in && half == 0) a.delta[((int64_t)b * a.H + h) * a.Lq + i] = s;
 }
@@ -847,11 +886,12 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq
   const int64_t stat = ((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i;
   const float lse = in ? a.lse[stat] : -INFINITY;
   float delta = 0.f;
-  {
+  for (const void* part : {a.o, a.o_rest}) {
+    if (!part) continue;
     typename M::frag o[NC];
     load_rows<T, M, DP>(o,
-                        static_cast<const T*>(a.o) + (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) *
-                                                         a.D,
+                        static_cast<const T*>(part) + (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) *
+                                                          a.D,
                         in, a.D, lane);
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -1116,6 +1156,7 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(XArgs a, int kind) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------
+constexpr int FINE_KEYS = 256;
 constexpr int FEW_ROWS = 8;  // rows of a key head that the single-token kernel takes
 
 // Blocks along one axis and shares of the other: where the tiles alone leave the chip idle, the
@@ -1262,7 +1303,14 @@ int xattn_forward(XArgs a, const XPlan& p, hipStream_t s) {
     typedef typename MmaOf<T>::type M;
     MPR_TRY(by_tile(a.D, p.fwd.nw, [&](auto dp, auto nw) -> int {
       constexpr int DP = dp, WR = nw;
-      xattn_fwd_kernel<T, M, DP, WR><<<blocks, 64 * NW, 0, s>>>(a);
+      // Where one key carries a row, P's rounding reaches the output and the backward's row sum at
+      // full size, where many do it averages out: at 2 keys, gradients 1.7 times as far off as their
+      // own rounding takes them, 1.45 times with P to 16 bits.  So few keys are multiplied FINE
+      // (2048 rows x 256 keys, 96 heads of 64: 42 us against 36).
+      if (std::is_same_v<T, bf16> && a.Lk <= FINE_KEYS)
+        xattn_fwd_kernel<T, M, DP, WR, std::is_same_v<T, bf16>><<<blocks, 64 * NW, 0, s>>>(a);
+      else
+        xattn_fwd_kernel<T, M, DP, WR, false><<<blocks, 64 * NW, 0, s>>>(a);
       MPR_LAUNCHED();
       return MPR_OK;
     }));
@@ -1332,8 +1380,8 @@ int mpr_xattn_workspace(const int64_t* dims, int32_t dtype, int64_t* fwd_bytes,
 }
 
 int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
-                  const int64_t* dims, const int64_t* strides, float scale, void* out, float* lse,
-                  void* ws, int64_t ws_bytes, void* stream) {
+                  const int64_t* dims, const int64_t* strides, float scale, void* out, void* rest,
+                  float* lse, void* ws, int64_t ws_bytes, void* stream) {
   return ops_call("xattn_fwd", [&]() -> int {
     MPR_TRY(xattn_check("xattn_fwd", dims, dtype));
     MPR_REQUIRE(strides && scale >= 0.f, "xattn_fwd: no strides, or a scale below 0");
@@ -1350,6 +1398,7 @@ int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* ke
                 "xattn_fwd: heads of k or v not at multiples of 4 bytes");
     XArgs a = xattn_args(q, k, v, keep, dims, strides, scale);
     a.out = out;
+    a.rest = dtype == MPR_BF16 ? rest : nullptr;
     a.lse = lse;
     a.part = static_cast<float*>(ws);
     a.part_ms = reinterpret_cast<float*>(static_cast<char*>(ws) + p.part_ms);
@@ -1361,7 +1410,7 @@ int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* ke
 
 int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* keep, int32_t dtype,
                   const int64_t* dims, const int64_t* strides, float scale, const void* out,
-                  const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
+                  const void* rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, void* ws,
                   int64_t ws_bytes, void* stream) {
   return ops_call("xattn_bwd", [&]() -> int {
     MPR_TRY(xattn_check("xattn_bwd", dims, dtype));
@@ -1382,6 +1431,7 @@ int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* ke
                 "xattn_bwd: heads not at multiples of 4 bytes");
     XArgs a = xattn_args(q, k, v, keep, dims, strides, scale);
     a.o = out;
+    a.o_rest = dtype == MPR_BF16 ? rest : nullptr;
     a.lse = const_cast<float*>(lse);
     a.dout = dout;
     a.do_bs = strides[10]; a.do_ls = strides[11]; a.do_hs = strides[12];

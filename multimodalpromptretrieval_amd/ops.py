@@ -208,66 +208,63 @@ def _heads(t):
     return t.contiguous() if not t.is_contiguous() else t.clone()
 
 
-def _xattn_dims(q, k):
-    B, Lq, H, D = q.shape
-    return B, H, k.shape[2], Lq, k.shape[1], D
-
-
-def _xattn_strides(q, k, v, keep, dout=None):
-    s = [*q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
-         0 if keep is None else keep.stride(0)]
-    return _i64(*s, *(dout.stride()[:3] if dout is not None else (0, 0, 0)))
-
-
 @lru_cache(maxsize=4096)
-def _xattn_bytes(code, *dims):
+def _xattn_plan(code, q_shape, k_shape, q_st, k_st, v_st, keep_st, dout_st):
+    """(dims, strides as the library takes them, workspace bytes of a forward and of a backward)."""
+    B, Lq, H, D = q_shape
+    dims = _i64(B, H, k_shape[2], Lq, k_shape[1], D)
+    strides = _i64(*q_st[:3], *k_st[:3], *v_st[:3], keep_st, *dout_st[:3])
     fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
-    _lib.call("mpr_xattn_workspace", _i64(*dims), code, ctypes.byref(fwd), ctypes.byref(bwd))
-    return fwd.value, bwd.value
+    _lib.call("mpr_xattn_workspace", dims, code, ctypes.byref(fwd), ctypes.byref(bwd))
+    return dims, strides, fwd.value, bwd.value
 
 
-def _xattn_fwd(q, k, v, keep, scale, want_lse):
-    code, dims = _DTYPES[q.dtype], _xattn_dims(q, k)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = None
-    if want_lse:
-        B, Lq, H, _ = q.shape
-        lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
-    nbytes, _ = _xattn_bytes(code, *dims)
+def _xattn_fwd(q, k, v, keep, scale, for_grad):
+    """(out, what rounding took off it (bf16), the rows' statistic), the latter two for_grad."""
+    code, shape = _DTYPES[q.dtype], q.shape
+    dims, strides, nbytes, _ = _xattn_plan(
+        code, shape, k.shape, q.stride(), k.stride(), v.stride(),
+        0 if keep is None else keep.stride(0), (0, 0, 0))
+    out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    rest = lse = None
+    if for_grad:
+        lse = torch.empty((shape[0], shape[2], shape[1]), dtype=torch.float32, device=q.device)
+        rest = torch.empty_like(out) if code == 1 else None
     ws = _workspace(nbytes, q.device)
-    _call(q.device, "mpr_xattn_fwd", _ptr(q), _ptr(k), _ptr(v), _ptr(keep), code,
-          _i64(*dims), _xattn_strides(q, k, v, keep), scale, _ptr(out), _ptr(lse), _ptr(ws),
-          nbytes)
-    return out, lse
+    _call(q.device, "mpr_xattn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(keep), code,
+          dims, strides, scale, out.data_ptr(), _ptr(rest), _ptr(lse), _ptr(ws), nbytes)
+    return out, rest, lse
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, keep, scale):
         q, k, v = _heads(q), _heads(k), _heads(v)
-        out, lse = _xattn_fwd(q, k, v, keep, scale, True)
-        ctx.save_for_backward(q, k, v, keep, out, lse)
+        out, rest, lse = _xattn_fwd(q, k, v, keep, scale, True)
+        ctx.save_for_backward(q, k, v, keep, out, rest, lse)
         ctx.scale = scale
         return out
 
     @staticmethod
     @_first_order
     def backward(ctx, dout):
-        q, k, v, keep, out, lse = ctx.saved_tensors
+        q, k, v, keep, out, rest, lse = ctx.saved_tensors
         dout = _heads(dout)
-        code, dims = _DTYPES[q.dtype], _xattn_dims(q, k)
+        code = _DTYPES[q.dtype]
+        dims, strides, _, nbytes = _xattn_plan(
+            code, q.shape, k.shape, q.stride(), k.stride(), v.stride(),
+            0 if keep is None else keep.stride(0), dout.stride())
         need_q, need_k, need_v = ctx.needs_input_grad[:3]
 
         def like(t, wanted):
             return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None
         dq = like(q, need_q)
-        dk, dv = (like(t, need_k or need_v) for t in (k, v))
-        _, nbytes = _xattn_bytes(code, *dims)
+        dk = like(k, need_k or need_v)
+        dv = like(v, need_k or need_v)
         ws = _workspace(nbytes, q.device)
-        _call(q.device, "mpr_xattn_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(keep),
-              code, _i64(*dims), _xattn_strides(q, k, v, keep, dout), ctx.scale, _ptr(out),
-              _ptr(lse), _ptr(dout), _ptr(dq), _ptr(dk), _ptr(dv),
-              _ptr(ws), nbytes)
+        _call(q.device, "mpr_xattn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(keep), code,
+              dims, strides, ctx.scale, out.data_ptr(), _ptr(rest), lse.data_ptr(),
+              dout.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(ws), nbytes)
         return dq, dk if need_k else None, dv if need_v else None, None, None
 
 
@@ -338,31 +335,39 @@ def _label_ids(logits, labels, what):
     return _tokens(labels, logits.device, what + " labels", logits.shape[2], -2 ** 63)
 
 
+@lru_cache(maxsize=4096)
+def _logps_plan(S, T, V):
+    """(bytes of the rows' statistics, of dlogps after them, of the workspace at the end)."""
+    return 8 * S * T, (4 * S + 7) // 8 * 8, _bytes("mpr_logps_workspace", S, T, V)
+
+
 def _logps_fwd(logits, labels, pair):
-    """(logps, row_stat, loss, dlogps); pair: (ref, beta, label_smoothing) or None."""
+    """(logps, loss, kept); kept: a buffer with the rows' statistics and the loss's derivative by
+    logps (and the workspace).  pair: (ref, beta, label_smoothing) or None."""
     S, T, V = logits.shape
     dev = logits.device
-
-    def f32(*shape):
-        return torch.empty(shape, dtype=torch.float32, device=dev)
-    logps, stat = f32(S), f32(S, T, 2)
-    loss, dlogps = (f32(), f32(S)) if pair else (None, None)
+    n_stat, n_dlp, n_ws = _logps_plan(S, T, V)
+    logps = torch.empty(S, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev) if pair else None
+    kept = torch.empty(n_stat + n_dlp + n_ws, dtype=torch.uint8, device=dev)
     ref, beta, smooth = pair or (None, 0.0, 0.0)
-    nbytes = _bytes("mpr_logps_workspace", S, T, V)
-    ws = _workspace(nbytes, dev)
-    _call(dev, "mpr_logps_fwd", _ptr(logits), _DTYPES[logits.dtype], S, T, V,
-          logits.stride(0), logits.stride(1), _ptr(labels), _IDS[labels.dtype], T,
-          _ptr(logps), _ptr(stat), _ptr(ref), beta, smooth, _ptr(loss),
-          _ptr(dlogps), _ptr(ws), nbytes)
-    return logps, stat, loss, dlogps
+    at = kept.data_ptr()
+    _call(dev, "mpr_logps_fwd", logits.data_ptr(), _DTYPES[logits.dtype], S, T, V,
+          logits.stride(0), logits.stride(1), labels.data_ptr(), _IDS[labels.dtype], T,
+          logps.data_ptr(), at, _ptr(ref), beta, smooth, _ptr(loss),
+          at + n_stat if pair else None, at + n_stat + n_dlp, n_ws)
+    return logps, loss, kept
 
 
-def _logps_bwd(logits, labels, stat, dlogps, mult):
+def _logps_bwd(logits, labels, kept, dlogps, mult):
+    """dlogps None: the loss's, which the forward kept."""
     S, T, V = logits.shape
     dx = torch.empty((S, T, V), dtype=logits.dtype, device=logits.device)
-    _call(logits.device, "mpr_logps_bwd", _ptr(logits), _DTYPES[logits.dtype], S, T, V,
-          logits.stride(0), logits.stride(1), _ptr(labels), _IDS[labels.dtype], T,
-          _ptr(stat), _ptr(dlogps), _ptr(mult), _ptr(dx))
+    at = kept.data_ptr()
+    _call(logits.device, "mpr_logps_bwd", logits.data_ptr(), _DTYPES[logits.dtype], S, T, V,
+          logits.stride(0), logits.stride(1), labels.data_ptr(), _IDS[labels.dtype], T, at,
+          at + _logps_plan(S, T, V)[0] if dlogps is None else dlogps.data_ptr(), _ptr(mult),
+          dx.data_ptr())
     return dx
 
 
@@ -370,32 +375,31 @@ class _SequenceLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels):
         logits = _rows(logits)
-        logps, stat, _, _ = _logps_fwd(logits, labels, None)
-        ctx.save_for_backward(logits, labels, stat)
+        logps, _, kept = _logps_fwd(logits, labels, None)
+        ctx.save_for_backward(logits, labels, kept)
         return logps
 
     @staticmethod
     @_first_order
     def backward(ctx, dlogps):
-        logits, labels, stat = ctx.saved_tensors
-        return _logps_bwd(logits, labels, stat, dlogps.contiguous(), None), None
+        logits, labels, kept = ctx.saved_tensors
+        return _logps_bwd(logits, labels, kept, dlogps.contiguous(), None), None
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ref, beta, smooth):
         logits = _rows(logits)
-        logps, stat, loss, dlogps = _logps_fwd(logits, labels, (ref, beta, smooth))
-        ctx.save_for_backward(logits, labels, stat, dlogps)
+        logps, loss, kept = _logps_fwd(logits, labels, (ref, beta, smooth))
+        ctx.save_for_backward(logits, labels, kept)
         ctx.mark_non_differentiable(logps)
         return loss, logps
 
     @staticmethod
     @_first_order
     def backward(ctx, dloss, _):
-        logits, labels, stat, dlogps = ctx.saved_tensors
-        return (_logps_bwd(logits, labels, stat, dlogps, dloss.contiguous()), None, None, None,
-                None)
+        logits, labels, kept = ctx.saved_tensors
+        return _logps_bwd(logits, labels, kept, None, dloss), None, None, None, None
 
 
 def sequence_logps(logits, labels):
@@ -440,7 +444,7 @@ def preference_loss(logits, labels, ref_logps, beta: float = 0.1, label_smoothin
     ref = ref_logps.detach().to(torch.float32).contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
         return _PreferenceLoss.apply(logits, labels, ref, beta, smooth)
-    logps, _, loss, _ = _logps_fwd(_rows(logits), labels, (ref, beta, smooth))
+    logps, loss, _ = _logps_fwd(_rows(logits), labels, (ref, beta, smooth))
     return loss, logps
 
 

@@ -75,7 +75,10 @@ def attention(q, k, v, keep, scale, dout=None):
     products are exact in fp32).
       out: sum_j p |v| (e + r + Lk u)
       dV:  sum_i p |dO| (e + r + R u), R rows
-      dS:  x = p ((e + r) |dP - delta| + D u sum |dO||v| + d_delta), d_delta = sum |dO| out's bound
+      dS:  x = p ((e + r) |dP - delta| + D u sum |dO||v| + d_delta).  delta is sum |dO O| of an O whose
+           weights w add up to 1 whatever their errors, so sum (w - p) dP = sum (w - p) (dP - delta)
+           and w - p is at most 2 (e + r) p: d_delta = 2 (e + r) sum p |dP - delta| + (D u + r^2 + u)
+           sum |dO O|, O itself being kept to two bf16 (r^2)
       dQ:  scale sum_j (x + p |dP - delta| Lk u) |k|;   dK with R and |q|
     fp32 has no normal number under 2^-126: exp2 of less than -126 may come out 0, and so may a
     product's operand or sum below it, so every p carries 2^-125 besides (two such steps): `least`."""
@@ -122,8 +125,8 @@ def attention(q, k, v, keep, scale, dout=None):
     dp = mm(do, t_(vv))
     delta = (do * out).sum(-1, keepdim=True)
     g = torch.where(live & some, p * (dp - delta), 0.0)
-    d_delta = (do.abs() * b_out).sum(-1, keepdim=True) + D * U * (do * out).abs().sum(
-        -1, keepdim=True)
+    spread = (p * (dp - delta).abs()).sum(-1, keepdim=True)
+    d_delta = 2 * (e + r) * spread + (D * U + r * r + U) * (do * out).abs().sum(-1, keepdim=True)
     x = (p * (e + r) + least) * (dp - delta).abs() + p * (
         D * U * mm(do.abs(), t_(vv.abs())) + d_delta)
     dq = scale * mm(g, kk)

@@ -141,6 +141,9 @@ def xattn_check(q, k, v, keep, scale, dout):
     (1, 4, 2, 130, 257, 128),
     (1, 16, 2, 17, 1000, 80),
     (4, 1, 1, 5, 2000, 120),
+    (3, 2, 1, 20, 1, 64),      # one key: no gradient reaches q or k
+    (7, 1, 1, 83, 2, 80),      # two: dP - rowsum(dO O) cancels
+    (2, 2, 2, 300, 3, 128),
 ])
 def test_cross_attention(device, dtype, B, H, Hkv, Lq, Lk, D):
     g = gen(Lq * 1000 + Lk)

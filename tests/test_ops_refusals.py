@@ -146,13 +146,31 @@ def test_c_entries_refuse_bad_arguments():
     refused("mpr_xattn_workspace", None, 0, out, out)
     refused("mpr_xattn_workspace", i64(*good), 7, out, out)
     st = i64(*[64] * 13)
-    refused("mpr_xattn_fwd", None, P, P, None, 0, i64(*good), st, 1.0, P, P, None, 0, None)
-    refused("mpr_xattn_fwd", P, P, P, None, 0, i64(*good), None, 1.0, P, P, None, 0, None)
-    refused("mpr_xattn_bwd", P, P, P, None, 0, i64(*good), st, 1.0, P, None, P, P, P, P, P,
-            1 << 40, None)
-    refused("mpr_xattn_bwd", P, P, P, None, 0, i64(*good), st, 1.0, P, P, P, P, P, None, P,
-            1 << 40, None)
-    refused("mpr_xattn_bwd", P, P, P, None, 0, i64(*good), st, 1.0, P, P, P, P, P, P, P, 8, None)
+
+    def fwd(q=P, k=P, strides=st, dtype=0, dims=good, scale=1.0, ws=P, ws_bytes=1 << 40):
+        refused("mpr_xattn_fwd", q, k, P, None, dtype, i64(*dims), strides, scale, P, None, P, ws,
+                ws_bytes, None)
+
+    def bwd(k=P, dtype=0, dims=good, lse=P, dv=P, strides=st, ws_bytes=1 << 40):
+        refused("mpr_xattn_bwd", P, k, P, None, dtype, i64(*dims), strides, 1.0, P, None, lse, P, P,
+                P, dv, P, ws_bytes, None)
+    many = (2, 4, 2, 30, 5, 64)
+    odd, off = i64(*[63] * 13), ctypes.c_void_p(4098)
+    fwd(q=None)
+    fwd(strides=None)
+    fwd(scale=-1.0)
+    fwd(scale=float("nan"))
+    fwd(dims=(1, 1, 1, 1, 1 << 20, 64), ws_bytes=8)  # split keys need a workspace
+    fwd(dims=(1, 1, 1, 1, 1 << 20, 64), ws=None)
+    fwd(dims=many, dtype=2)  # float16 beyond single tokens
+    fwd(dims=many, dtype=1, strides=odd)  # bf16 heads at odd elements
+    fwd(dims=many, k=off)
+    bwd(lse=None)
+    bwd(dv=None)
+    bwd(ws_bytes=8)
+    bwd(dtype=2)
+    bwd(dtype=1, strides=odd)
+    bwd(k=off)
     refused("mpr_logps_workspace", 2, 3, 0, out)
     refused("mpr_logps_workspace", 1 << 20, 1 << 20, 5, out)
     refused("mpr_logps_workspace", 2, 3, 4, None)
