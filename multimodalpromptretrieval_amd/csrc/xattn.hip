@@ -380,20 +380,29 @@ __device__ __forceinline__ RowAt row_at(const XArgs& a, int hk, int r) {
   return {hk * a.G + g, r - g * a.Lq};
 }
 
-// Which (tile, split, batch, key head) a block computes.  Blocks go round robin over the 8 XCDs, so
-// neighbours in the order below, which read the same keys, are given to one XCD and its L2.
+// Which (tile, split, batch, key head) a block computes.  Blocks go round robin over the 8 XCDs; the
+// tiles of one split of a key head read the same keys, so they are given to one XCD and its L2, and
+// neighbouring key heads to different XCDs: the heads of a batch entry have its length in common, and
+// with whole entries on an XCD the longest one's would keep the others waiting.
 struct Job {
   int tile, split, b, hk;
   int64_t bh;
 };
 __device__ __forceinline__ Job job_of(const XArgs& a) {
-  const uint32_t n = gridDim.x, x = blockIdx.x % 8, q = n / 8, r = n % 8;
-  const uint32_t id = x * q + min(x, r) + blockIdx.x / 8;
+  const uint32_t groups = gridDim.x / a.tiles, even = groups / 8 * 8, at = blockIdx.x;
+  uint32_t group;
   Job j;
-  j.tile = id % a.tiles;
-  const uint32_t rest = id / a.tiles;
-  j.split = rest % a.splits;
-  j.bh = rest / a.splits;
+  if (at < even * a.tiles) {
+    const uint32_t i = at / 8;
+    group = i / a.tiles * 8 + at % 8;
+    j.tile = i % a.tiles;
+  } else {
+    const uint32_t i = at - even * a.tiles;
+    group = even + i / a.tiles;
+    j.tile = i % a.tiles;
+  }
+  j.split = group % a.splits;
+  j.bh = group / a.splits;
   j.b = (int)(j.bh / a.Hkv);
   j.hk = (int)(j.bh % a.Hkv);
   return j;
