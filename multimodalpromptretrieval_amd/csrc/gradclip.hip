@@ -222,7 +222,7 @@ int clip_check(int n, const int64_t* desc) {
   spans.reserve(2 * (size_t)n);
   for (int i = 0; i < n; ++i) {
     const int64_t* d = desc + 5 * (int64_t)i;
-    MPR_REQUIRE(d[1] >= 0 && d[1] <= (int64_t)1 << 40, "clip_grads: tensor %d has %lld values", i,
+    MPR_REQUIRE(d[1] >= 0 && d[1] <= (int64_t)1 << 37, "clip_grads: tensor %d has %lld values", i,
                 (long long)d[1]);
     MPR_REQUIRE(d[2] >= 0 && d[2] <= 2 && (!d[3] || (d[4] >= 0 && d[4] <= 2)),
                 "clip_grads: tensor %d has dtype codes %lld, %lld", i, (long long)d[2],

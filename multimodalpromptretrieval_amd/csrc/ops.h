@@ -97,6 +97,7 @@ int ops_call(const char* what, F&& f) {
 }
 inline hipStream_t op_stream(void* s) { return reinterpret_cast<hipStream_t>(s); }
 
-constexpr int64_t MAX_GRID_X = 0x7FFFFFFF;
+// A launch has less than 2^32 threads along x: blocks of up to 512 threads.
+constexpr int64_t MAX_GRID_X = ((int64_t)1 << 23) - 1;
 
 }  // namespace mpr

@@ -500,7 +500,7 @@ template <class T, class M, int DP, int WR, bool FINE>
 __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fwd_kernel(XArgs a) {
   typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
-  constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK;
   __shared__ __align__(16) char lds[S::BYTES];
   __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
   __shared__ uint32_t words[SPAN / 32];
@@ -870,7 +870,7 @@ template <class T, class M, int DP, int WR>
 __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq_kernel(XArgs a) {
   typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
-  constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK;
   __shared__ __align__(16) char lds[S::BYTES];
   __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
   __shared__ uint32_t words[SPAN / 32];
@@ -975,7 +975,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WC>::BWD_OCC)) void xattn_dk
   typedef DkvShape<M, DP, WC> S;
   typedef typename M::elem E;
   constexpr int RT = S::RT, WS = S::WS, NU = S::NU;
-  constexpr int NC = DP / M::CHUNK, PC = 32 / M::CHUNK;
+  constexpr int NC = DP / M::CHUNK;
   __shared__ __align__(16) char lds[S::BYTES];
   __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
   // -lse (-inf: a row without a key), then delta, of the tile's rows

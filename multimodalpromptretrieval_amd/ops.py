@@ -33,7 +33,7 @@ import ctypes
 import math
 from array import array
 from functools import lru_cache
-from operator import attrgetter
+from operator import attrgetter, index
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -185,9 +185,10 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
     V = weight.shape[0]
     pad = -1
     if padding_idx is not None:
+        padding_idx = index(padding_idx)
         if not -V <= padding_idx < V:
             raise ValueError(f"embed: padding_idx {padding_idx} in a table of {V} rows")
-        pad = int(padding_idx) % V
+        pad = padding_idx % V
     scale = float(scale)
     ids = _tokens(ids, weight.device, "embed ids", V, 0)
     if weight.requires_grad and torch.is_grad_enabled():
@@ -196,6 +197,7 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
 
 
 # ---- cross attention -----------------------------------------------------------------------------
+_MOST_SCALE = 2.0 ** 120  # times log2(e), it is still a float32
 _FEW_ROWS = 8  # rows of a key head that the single-token kernel takes, in any type
 
 
@@ -205,7 +207,8 @@ def _heads(t):
     if d == 1 and (t.dtype == torch.float32 or
                    not ((b | l | h) & 1 or t.data_ptr() & 3)):
         return t
-    return t.contiguous() if not t.is_contiguous() else t.clone()
+    # (a copy made by clone or contiguous may keep an odd stride of a dimension of size 1)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
 @lru_cache(maxsize=4096)
@@ -295,7 +298,7 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
     if D < 8 or D > 128 or D % 8:
         raise ValueError(f"cross_attention: head dim {D} (a multiple of 8 up to 128)")
     scale = float(scale)
-    if not math.isfinite(scale):
+    if not abs(scale) <= _MOST_SCALE:
         raise ValueError(f"cross_attention: scale {scale}")
     keep = None
     if key_mask is not None:
@@ -504,6 +507,10 @@ def _check_outs(grads, out, what):
     return codes
 
 
+def _listed(tensors):
+    return [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+
+
 def _clip(grads, out, max_norm, eps, what):
     n = len(grads)
     if out is not None and len(out) != n:
@@ -539,9 +546,9 @@ def _clip(grads, out, max_norm, eps, what):
 
 @torch.no_grad()
 def grad_norm(grads):
-    """The L2 norm of all values of the tensors together (a float32 scalar on their device; 0 on the
-    host for none).  Squares are summed in 64 bits."""
-    return _clip(list(grads), None, None, 0.0, "grad_norm")
+    """The L2 norm of all values of the tensors (or the one tensor) together: a float32 scalar on their
+    device, 0 on the host for none.  Squares are summed in 64 bits."""
+    return _clip(_listed(grads), None, None, 0.0, "grad_norm")
 
 
 @torch.no_grad()
@@ -550,15 +557,16 @@ def clip_grads_(grads, max_norm: float, eps: float = 1e-6, out=None):
     global L2 norm before it (``grad_norm``).
 
     In place, or into ``out``: a tensor for each gradient, of its shape (or, both contiguous, its
-    number of values) and any floating type (the optimizer's fp32 buffer for bf16 gradients).  Gradients below the limit are not written in
-    place at all.  The types may differ between tensors.  A norm that is not finite goes through as
+    number of values) and any floating type (the optimizer's fp32 buffer for bf16 gradients).
+    Gradients below the limit are not written in place at all.  The types may differ between
+    tensors, and one tensor alone needs no list.  A norm that is not finite goes through as
     it is: NaN makes every gradient NaN, infinity makes finite ones 0.  Tensors that share memory
     (one gradient listed twice) and gradients with gaps in their memory are refused."""
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0.0 or not eps >= 0.0:
         raise ValueError(f"clip_grads_: max_norm {max_norm}, eps {eps}")
-    grads = list(grads)
-    out = None if out is None else list(out)
+    grads = _listed(grads)
+    out = None if out is None else _listed(out)
     norm = _clip(grads, out, max_norm, eps, "clip_grads_")
     if grads:
         torch.autograd.graph.increment_version(grads if out is None else out)

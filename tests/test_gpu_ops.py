@@ -213,6 +213,19 @@ def test_cross_attention_strides(device, dtype):
     xattn_check(q[:, :1], k, v, keep, 0.3, dout[:, :1])
 
 
+@pytest.mark.parametrize("Lq", [1, 12])
+def test_cross_attention_odd_strides_of_single_dims(device, Lq):
+    """A dimension of size 1 has whatever stride it came with; an odd one is nobody's address."""
+    g = gen(13)
+    q = randn(g, 1, Lq, 1, 64, dtype=BF16)
+    k, v = (randn(g, 1, 70, 1, 64, dtype=BF16).as_strided((1, 70, 1, 64), (4481, 64, 7, 1))
+            for _ in range(2))
+    one = [t[:, :1].as_strided((1, 1, 1, 64), (65, 67, 7, 1)) for t in (k, v)]
+    dout = randn(g, 1, Lq, 1, 64, dtype=BF16).as_strided((1, Lq, 1, 64), (64 * Lq + 1, 64, 3, 1))
+    xattn_check(q, k, v, None, 0.2, dout)
+    xattn_check(q, *one, None, 0.2, dout)
+
+
 def test_cross_attention_large_scores(device):
     """Scores of hundreds: one key takes nearly all, and no exponent overflows."""
     g = gen(11)
@@ -440,6 +453,21 @@ def test_clip_layouts(device):
         ops.clip_grads_([a], 1.0, out=[torch.empty(50, 30, device="cuda")])
 
 
+def test_clip_one_tensor(device):
+    """A tensor alone, its rows not being the list."""
+    g = gen(34)
+    x = randn(g, 6, 50)
+    keep = x.clone()
+    norm, c = clip_want([keep], 0.1)
+    assert ops.grad_norm(x).item() == pytest.approx(float(norm), rel=1e-6)
+    out = torch.empty(300, device="cuda")
+    ops.clip_grads_(x, 0.1, out=out)
+    assert torch.equal(x, keep)
+    clip_check(out.view(6, 50), keep, c, F32)
+    ops.clip_grads_(x, 0.1)
+    assert torch.equal(x, out.view(6, 50))
+
+
 def test_clip_same_bits_wherever_the_tensors_lie(device):
     g = gen(33)
     src = [randn(g, n) for n in (70001, 33, 5000)]
@@ -631,6 +659,17 @@ def test_embed_past_32_bits(device):
     dout[-50:] = 1.5
     dw, = torch.autograd.grad(out, w, dout)
     R.check(dw, *R.embed_grad(dout[-50:], ids[-50:], 50, 1.0, None, BF16))
+
+
+def test_embed_more_rows_than_a_launch_takes(device):
+    n = (1 << 27) + 77  # 4 x 4 rows a block: more than 2^23 - 1 blocks
+    w = randn(gen(104), 300, 1, dtype=BF16)
+    ids = torch.randint(0, 300, (n,), dtype=torch.int32, device="cuda", generator=gen(105))
+    got = ops.embed(w, ids)
+    assert got.shape == (n, 1)
+    for at in range(0, n, 1 << 24):
+        part = slice(at, min(n, at + (1 << 24)))
+        assert torch.equal(got[part, 0], w[:, 0][ids[part].long()])
 
 
 def test_cross_attention_past_32_bits(device):

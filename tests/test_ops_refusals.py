@@ -206,3 +206,22 @@ def test_workspaces_grow_with_the_work():
     _lib.call("mpr_xattn_workspace", i64(4, 16, 4, 1024, 4096, 128), 1, ctypes.byref(fwd),
               ctypes.byref(bwd))
     assert bwd.value >= 4 * 16 * 1024 * 4
+
+
+def test_numbers_out_of_range():
+    q, k = T(2, 3, 4, 64), T(2, 5, 2, 64)
+    for scale in (1e39, -1e39, 2.0 ** 121):  # float32 of these, times log2(e), is not finite
+        with pytest.raises(ValueError, match="scale"):
+            ops.cross_attention(q, k, k, scale=scale)
+    for pad in (1.5, "1"):  # not a row of the table
+        with pytest.raises(TypeError):
+            ops.embed(T(5, 4), T(3, dtype=torch.int64), padding_idx=pad)
+
+
+def test_clip_one_tensor_is_not_its_rows():
+    with pytest.raises(ValueError, match="1 gradients and 2 outputs"):
+        ops.clip_grads_(T(3, 4), 1.0, out=[T(4), T(4)])
+    with pytest.raises(ValueError, match="GPU"):
+        ops.clip_grads_(T(3, 4), 1.0, out=T(3, 4))
+    with pytest.raises(ValueError, match="GPU"):
+        ops.grad_norm(T(()))
