@@ -612,25 +612,46 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
     a.lse[((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m * a.c + log2f(l);
 }
 
-// The splits of a row: rescaled to their common maximum and summed in order.  A wave per row.
+// The splits of a row: rescaled to their common maximum and summed in order.  A wave per row, whose
+// lanes read the splits' statistics side by side and then AHEAD of their rows at a time: the time is
+// the latency of these reads (1024 rows of 4 splits 4.8 us; one split after the other 8.7).
 template <class T>
 __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
   const int lane = threadIdx.x & 63;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.R;
   const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= rows) return;
-  float m = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ms[2 * (s * rows + at)]);
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2* ms = reinterpret_cast<const f32x2*>(a.part_ms);
+  constexpr int AHEAD = 8;
+  const f32x2 none = {-INFINITY, 0.f};
+  const f32x2 first = lane < a.splits ? ms[lane * rows + at] : none;
+  float m = first[0];
+  for (int s = lane + 64; s < a.splits; s += 64) m = fmaxf(m, ms[s * rows + at][0]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[2] = {0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t p = s * rows + at;
-    const float w = exp2_fast(a.part_ms[2 * p] - base);
-    l += w * a.part_ms[2 * p + 1];
+  for (int s0 = 0; s0 < a.splits; s0 += 64) {  // a lane per split, for its weight
+    const int n = min(64, a.splits - s0);
+    const f32x2 x = s0 == 0 ? first : lane < n ? ms[(s0 + lane) * rows + at] : none;
+    const float w = exp2_fast(x[0] - base);
+    l += wave_add(w * x[1]);
+    for (int s = 0; s < n; s += AHEAD) {
+      float y[AHEAD][2];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int d = lane + 64 * j;
-      if (d < a.D) o[j] += w * a.part[p * a.D + d];
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int d = lane + 64 * j;
+          y[u][j] = s + u < n && d < a.D ? a.part[((s0 + s + u) * rows + at) * a.D + d] : 0.f;
+        }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const float f = __shfl(w, min(s + u, n - 1), 64);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) o[j] += f * y[u][j];
+      }
     }
   }
   const int64_t bh = at / a.R;
@@ -675,6 +696,17 @@ __device__ __forceinline__ float group_add(float x) {
   }
   return x;
 }
+// f over the lanes that hold the same column of neighbouring groups of LPR, in all of them
+template <int LPR, class F>
+__device__ __forceinline__ float across(float x, F f) {
+  if constexpr (LPR == 8) x = f(x, permuted<0x128>(x));  // turned by 8 within 16: lane ^ 8
+  if constexpr (LPR <= 16) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
+  }
+  return halves(x, f);
+}
 
 template <class T, int LPR, int NR>
 __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
@@ -685,8 +717,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
   __shared__ uint32_t words[SPAN / 32];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int split = blockIdx.x % a.splits;
-  const int64_t bh = blockIdx.x / a.splits;
+  // The first share of every head, then the second, ...: a head's last shares may lie behind its
+  // length, and with its shares side by side one XCD got all the last ones.  Each share begins with
+  // another head, so that a CU's blocks are of different batch entries.
+  const uint32_t heads = (uint32_t)(a.B * a.Hkv);
+  const int split = (int)(blockIdx.x / heads);
+  const int64_t bh = (blockIdx.x % heads + (uint64_t)split * heads / a.splits) % heads;
   const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
   const T* k = static_cast<const T*>(a.k) + b * a.k_bs + hk * a.k_hs;
   const T* v = static_cast<const T*>(a.v) + b * a.v_bs + hk * a.v_hs;
@@ -790,16 +826,13 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
   }
 #pragma unroll
   for (int r = 0; r < NR; ++r) {  // the wave's groups of lanes
+    const float top = across<LPR>(m[r], [](float x, float y) { return fmaxf(x, y); });
+    const float w = exp2_fast(m[r] - (top == -INFINITY ? 0.f : top));
+    const auto add = [](float x, float y) { return x + y; };
+    m[r] = top;
+    l[r] = across<LPR>(l[r] * w, add);
 #pragma unroll
-    for (int off = LPR; off < 64; off <<= 1) {
-      const float m2 = __shfl_xor(m[r], off, 64), l2 = __shfl_xor(l[r], off, 64);
-      const float top = fmaxf(m[r], m2), zero = top == -INFINITY ? 0.f : top;
-      const float w = exp2_fast(m[r] - zero), w2 = exp2_fast(m2 - zero);
-      m[r] = top;
-      l[r] = l[r] * w + l2 * w2;
-#pragma unroll
-      for (int e = 0; e < N; ++e) o[r][e] = o[r][e] * w + __shfl_xor(o[r][e], off, 64) * w2;
-    }
+    for (int e = 0; e < N; ++e) o[r][e] = across<LPR>(o[r][e] * w, add);
     if (lane < LPR)
 #pragma unroll
       for (int e = 0; e < N; ++e) so[wave][r][d0 + e] = o[r][e];
@@ -1199,7 +1232,10 @@ XPlan xattn_plan(const int64_t* dims) {
   XPlan p;
   p.few = R <= FEW_ROWS;
   if (p.few) {
-    p.fwd = tiling(heads, 1, Lk, 512, 1024, 64);
+    // One or two rows: two blocks a CU hide each other's beginning and end (160 heads of 4096 keys,
+    // D = 128 bf16: 43 us, with one a CU 48).  More rows keep the vector units busier than memory,
+    // and more shares only cost their joins (64 heads of 8192 keys, 4 rows: 52 us, with two 58).
+    p.fwd = tiling(heads, 1, Lk, R <= 2 ? 512 : 256, 512, 64);
     p.fwd.tiles = 1;
   } else {
     p.fwd = tiling(heads, R, Lk, 256, 256, 128);
