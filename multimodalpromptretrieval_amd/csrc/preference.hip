@@ -45,7 +45,9 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
   return {m, a.s * exp_from(a.m, m) + b.s * exp_from(b.m, m)};
 }
 
-// stat[row * split + part] = the maximum and sum over the part's columns
+// stat[row * split + part] = the maximum and sum over the part's columns.  Bound by the read of the
+// labelled rows: 8192 rows of 32128 in bf16, five eighths of them labelled (329 MB), 48 us, 6.9 TB/s
+// (part of them from the caches); 320 rows of 32101 in fp32 6.4 us.
 template <class T>
 __global__ __launch_bounds__(LP_THREADS) void lp_stats_kernel(const T* __restrict__ x, LpArgs a,
                                                               MaxSum* __restrict__ stat) {
@@ -162,7 +164,8 @@ __global__ __launch_bounds__(1024) void lp_pairs_kernel(const double* lp, const 
   lp_pairs(lp, ref, P, beta, eps, loss, dlp);
 }
 
-// Few sequences: both in one launch, a wave for each sequence in turn.
+// Few sequences: both in one launch, a wave for each sequence in turn (16 sequences of 20: 5 us, and a
+// launch of 3.4 us of host time less).
 constexpr int LP_FEW = 64;
 template <class T>
 __global__ __launch_bounds__(1024) void lp_few_kernel(const T* x, LpArgs a, const MaxSum* stat,
@@ -182,6 +185,9 @@ __global__ __launch_bounds__(1024) void lp_few_kernel(const T* x, LpArgs a, cons
   lp_pairs(lp64, ref, a.S / 2, beta, eps, loss, dlp);
 }
 
+// dx, a block per row (and part of it).  Bound by memory: labelled rows are read again, every row is
+// written; the exponentials hide behind that.  The 8192 rows above (329 MB in, 526 MB out) 150 us, 5.7
+// TB/s, with stores that pass the caches by (29 us more without: they push out logits still to be read).
 template <class T, bool STREAM>
 __global__ __launch_bounds__(LP_THREADS) void lp_grad_kernel(const T* __restrict__ x, LpArgs a,
                                                              const MaxSum* __restrict__ row_stat,

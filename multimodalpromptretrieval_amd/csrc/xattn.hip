@@ -496,6 +496,14 @@ __device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* word
 // The running maximum follows the scores only when they pass it by more than 8 (in base 2): until
 // then exponentials up to 2^8 share the old base, and the sums need no rescaling.
 // FINE: P to 16 bits as an operand (bf16).
+//
+// What bounds it are the matrix cores and the vector work of the exponentials (16 a lane for each 32 x 32
+// scores), which overlap little: at D = 128 the matrix pipes are busy 40 % of the cycles and the
+// vector pipes 43 %.  32 rows a wave hold Q, the scores and the sums in registers with two waves a
+// SIMD (three at D = 64); four waves along the rows read a staged tile of 64 keys four times.  4 x 16
+// heads over 4, 1024 x 4096 keys, D = 128 in bf16 156 to 175 us (790 to 880 TFLOP/s), D = 64 99 us
+// (700); in fp32, whose products take 16 times as long and hide the rest, 1022 us and 552 us (135 and
+// 125 of 154 TFLOP/s).
 template <class T, class M, int DP, int WR, bool FINE>
 __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fwd_kernel(XArgs a) {
   typedef Shape<M, DP, WR> S;
@@ -674,7 +682,10 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // for the mask's bits and the end.  LPR lanes read a key's row, 16 bytes each, so a wave reads 64 /
 // LPR keys at a time; each such group of lanes keeps its own running maximum, sum and output share
 // of every row, and they are joined when the keys are done.  The wave's next FEW_AHEAD reads are on
-// their way while the present ones are computed.
+// their way while the present ones are computed.  32 x 8 key heads of 4 rows, 8192 keys, D = 128 in
+// bf16: 199 us, 5.4 TB/s; 16 x 12 heads, 562 keys, D = 64 in fp32 9.6 us, half of it until the first
+// keys are there.  (Reading the first keys before the mask is known made masked batches slower, 66 us
+// against 60; blocks of 4 waves 207 us against 199.)
 constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
 
 template <int CTRL>
@@ -898,7 +909,11 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
   if (in && half == 0) a.delta[((int64_t)b * a.H + h) * a.Lq + i] = s;
 }
 
-// dQ: WR of the block's waves along the rows (32 each), the others along the staged keys.
+// dQ: WR of the block's waves along the rows (32 each), the others along the staged keys.  Scores and
+// dP come from one pass over K and V by rows, dS goes on to the third product in registers, and delta
+// is formed from O and dO while the first tile is on its way.  Three products for two of the forward's,
+// bound as it is: 4 x 16 heads over 4, 1024 x 4096, D = 128 in bf16 209 to 224 us (920 to 990 TFLOP/s
+// of its 6 B H Lq Lk D, where a large product reaches 1072).
 template <class T, class M, int DP, int WR>
 __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq_kernel(XArgs a) {
   typedef Shape<M, DP, WR> S;
@@ -989,7 +1004,10 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq
 }
 
 // dK, dV: WC of the block's waves along the keys (32 each), the others along the staged rows, RT at a
-// time, over the rows of every head that shares the keys.
+// time, over the rows of every head that shares the keys.  K and V are operands of every product and
+// dK and dV sums of all: at D = 128 V waits in LDS (V_LDS), the rest leaves two waves a SIMD in bf16
+// and one in fp32.  Four products: 4 x 16 heads over 4, 1024 x 4096, D = 128 in bf16 291 to 306 us (900 to
+// 940 TFLOP/s of its 8 B H Lq Lk D); with dQ in fp32 3683 us, 131 of 154 TFLOP/s.
 template <class M, int DP, int WC>
 struct DkvShape {
   typedef typename M::elem E;
