@@ -681,7 +681,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // The keys and values are read once and that is all the time there is: no matrix core, and LDS only
 // for the mask's bits and the end.  LPR lanes read a key's row, 16 bytes each, so a wave reads 64 /
 // LPR keys at a time; each such group of lanes keeps its own running maximum, sum and output share
-// of every row, and they are joined when the keys are done.  The wave's next FEW_AHEAD reads are on
+// of every row (the maximum moves as the tiled kernel's does), and they are joined when the keys are done.  The wave's next FEW_AHEAD reads are on
 // their way while the present ones are computed.  32 x 8 key heads of 4 rows, 8192 keys, D = 128 in
 // bf16: 199 us, 5.4 TB/s; 16 x 12 heads, 562 keys, D = 64 in fp32 9.6 us, half of it until the first
 // keys are there.  (Reading the first keys before the mask is known made masked batches slower, 66 us
@@ -719,6 +719,89 @@ __device__ __forceinline__ float across(float x, F f) {
   return halves(x, f);
 }
 
+// Sums of NR rows over the lanes of a group, one row to a lane: instead of NR sums in every lane, each
+// exchange halves the rows that a lane goes on with, so a score's exponential is taken once for every
+// 8 lanes' rows, not in each.  Row r is then held by lane lane_of<NR>(r) of every 8.
+template <int NR>
+constexpr int lane_of(int r) {
+  return NR == 1 ? 0 : NR == 2 ? 4 * r : NR == 4 ? 4 * (r >> 1) + (r & 1)
+                                                 : 4 * (r >> 2) + (r >> 1 & 1) + 2 * (r & 1);
+}
+template <int LPR, int NR>
+__device__ __forceinline__ float row_sums(const float (&y)[NR], int lane) {
+  if constexpr (NR == 1) {
+    return group_add<LPR>(y[0]);
+  } else {
+    const bool b0 = lane & 1, b1 = lane & 2, b2 = lane & 4;
+    float x, a[NR / 2];
+#pragma unroll
+    for (int i = 0; i < NR / 2; ++i)
+      a[i] = (b2 ? y[NR / 2 + i] : y[i]) + permuted<0x141>(b2 ? y[i] : y[NR / 2 + i]);
+    if constexpr (NR == 2) {
+      x = a[0] + permuted<0xB1>(a[0]);
+      x += permuted<0x4E>(x);
+    } else if constexpr (NR == 4) {
+      x = (b0 ? a[1] : a[0]) + permuted<0xB1>(b0 ? a[0] : a[1]);
+      x += permuted<0x4E>(x);
+    } else {
+      float b[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        b[i] = (b0 ? a[2 + i] : a[i]) + permuted<0xB1>(b0 ? a[i] : a[2 + i]);
+      x = (b1 ? b[1] : b[0]) + permuted<0x4E>(b1 ? b[0] : b[1]);
+    }
+    if constexpr (LPR >= 16) x += permuted<0x128>(x);  // lane ^ 8
+    if constexpr (LPR == 32) {
+      const uint32_t u = __builtin_bit_cast(uint32_t, x);
+      const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+      x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+    }
+    return x;
+  }
+}
+// and back: the value of every row in every lane of the group
+template <int LPR, int NR, int R = 0>
+__device__ __forceinline__ void row_values(float x, float lo, float hi, float (&all)[NR]) {
+  constexpr int L = lane_of<NR>(R);
+  if constexpr (LPR == 8) all[R] = permuted<(L & 3) * 0x55>(L & 4 ? hi : lo);
+  else all[R] = permuted<0x150 + L>(x);  // lane L of the 16 to all of them
+  if constexpr (R + 1 < NR) row_values<LPR, NR, R + 1>(x, lo, hi, all);
+}
+template <int LPR, int NR>
+__device__ __forceinline__ void row_values(float x, int lane, float (&all)[NR]) {
+  if constexpr (NR == 1) {
+    all[0] = x;
+  } else {
+    float lo = x, hi = x;  // of 8 lanes, the lower four's values and the upper four's
+    if constexpr (LPR == 8) {
+      const float down = permuted<0x124>(x), up = permuted<0x12C>(x);  // from lane - 4, lane + 4
+      lo = lane & 4 ? down : x;
+      hi = lane & 4 ? x : up;
+    }
+    row_values<LPR, NR, 0>(x, lo, hi, all);
+  }
+}
+
+// The dot product of two 16-byte runs (of 2-byte types in exact pair products), from `x` on.
+template <class T>
+__device__ __forceinline__ float dot16(const typename Vec<T, VEC16<T>>::type& a,
+                                       const typename Vec<T, VEC16<T>>::type& b, float x) {
+  if constexpr (sizeof(T) == 2) {
+    typedef T pair __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      if constexpr (std::is_same_v<T, bf16>)
+        x = __builtin_amdgcn_fdot2_f32_bf16(pair{a[e], a[e + 1]}, pair{b[e], b[e + 1]}, x, false);
+      else
+        x = __builtin_amdgcn_fdot2(pair{a[e], a[e + 1]}, pair{b[e], b[e + 1]}, x, false);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x = fmaf(a[e], b[e], x);
+  }
+  return x;
+}
+
 template <class T, int LPR, int NR>
 __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
   constexpr int N = VEC16<T>, KPI = 64 / LPR, GROUP = KPI * FEW_AHEAD, STEP = FEW_WAVES * GROUP;
@@ -740,19 +823,18 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
   const uint8_t* keep = a.keep ? a.keep + b * a.keep_bs : nullptr;
   const int d0 = (lane % LPR) * N, sub = lane / LPR;
   const bool act = d0 < a.D;
-  float q[NR][N], o[NR][N], m[NR], l[NR];
+  typedef typename Vec<T, N>::type Run;
+  Run q[NR];
+  float o[NR][N], m = -INFINITY, l = 0.f;  // m, l: of the lane's row, unscaled scores
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
+    q[r] = Run{};
 #pragma unroll
-    for (int e = 0; e < N; ++e) q[r][e] = o[r][e] = 0.f;
+    for (int e = 0; e < N; ++e) o[r][e] = 0.f;
     if (r < a.R && act) {
       const RowAt ra = row_at(a, hk, r);
-      load_f<T, N>(static_cast<const T*>(a.q) + b * a.q_bs + ra.i * a.q_ls + ra.h * a.q_hs + d0,
-                   q[r]);
-#pragma unroll
-      for (int e = 0; e < N; ++e) q[r][e] *= a.c;
+      q[r] = *reinterpret_cast<const Run*>(static_cast<const T*>(a.q) + b * a.q_bs +
+                                           ra.i * a.q_ls + ra.h * a.q_hs + d0);
     }
   }
   struct Ahead {
@@ -782,44 +864,40 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
       }
     };
     const auto take = [&](const Ahead& x) {
-      float s[NR][FEW_AHEAD];
+      float s[FEW_AHEAD], top = m;
 #pragma unroll
       for (int u = 0; u < FEW_AHEAD; ++u) {
-        float f[N];
+        float y[NR];
 #pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = vec_f<T, N>(x.k[u], e);
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float y = 0.f;
-#pragma unroll
-          for (int e = 0; e < N; ++e) y = fmaf(q[r][e], f[e], y);
-          y = group_add<LPR>(y);
-          s[r][u] = x.ok[u] ? y : -INFINITY;
-        }
+        for (int r = 0; r < NR; ++r) y[r] = dot16<T>(q[r], x.k[u], 0.f);
+        const float z = row_sums<LPR, NR>(y, lane);
+        s[u] = x.ok[u] ? z : -INFINITY;
+        top = fmaxf(top, s[u]);
       }
-#pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        float top = m[r];
-#pragma unroll
-        for (int u = 0; u < FEW_AHEAD; ++u) top = fmaxf(top, s[r][u]);
-        const float zero = top == -INFINITY ? 0.f : top;
-        const float alpha = exp2_fast(m[r] - zero);
-        m[r] = top;
-        l[r] *= alpha;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o[r][e] *= alpha;
-#pragma unroll
-        for (int u = 0; u < FEW_AHEAD; ++u) l[r] += s[r][u] = exp2_fast(s[r][u] - zero);
-      }
-#pragma unroll
-      for (int u = 0; u < FEW_AHEAD; ++u) {
-        float f[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) f[e] = vec_f<T, N>(x.v[u], e);
+      if (__ballot(top > m + a.slack)) {
+        float alpha[NR];
+        const float mine = top == -INFINITY ? 1.f : exp2_fast((m - top) * a.c);
+        m = top;
+        l *= mine;
+        row_values<LPR, NR>(mine, lane, alpha);
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < N; ++e) o[r][e] = fmaf(s[r][u], f[e], o[r][e]);
+          for (int e = 0; e < N; ++e) o[r][e] *= alpha[r];
+      }
+      const float zero = m == -INFINITY ? 0.f : -m * a.c;
+#pragma unroll
+      for (int u = 0; u < FEW_AHEAD; ++u) l += s[u] = exp2_fast(fmaf(s[u], a.c, zero));
+#pragma unroll
+      for (int u = 0; u < FEW_AHEAD; ++u) {
+        float f[N], p[NR];
+#pragma unroll
+        for (int e = 0; e < N; ++e) f[e] = vec_f<T, N>(x.v[u], e);
+        row_values<LPR, NR>(s[u], lane, p);
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int e = 0; e < N; ++e) o[r][e] = fmaf(p[r], f[e], o[r][e]);
       }
     };
     Ahead x, y;
@@ -835,21 +913,24 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
       take(y);
     }
   }
-#pragma unroll
-  for (int r = 0; r < NR; ++r) {  // the wave's groups of lanes
-    const float top = across<LPR>(m[r], [](float x, float y) { return fmaxf(x, y); });
-    const float w = exp2_fast(m[r] - (top == -INFINITY ? 0.f : top));
+  {  // the wave's groups of lanes
     const auto add = [](float x, float y) { return x + y; };
-    m[r] = top;
-    l[r] = across<LPR>(l[r] * w, add);
+    const float top = across<LPR>(m, [](float x, float y) { return fmaxf(x, y); });
+    const float mine = top == -INFINITY ? 1.f : exp2_fast((m - top) * a.c);
+    l = across<LPR>(l * mine, add);
+    float w[NR];
+    row_values<LPR, NR>(mine, lane, w);
 #pragma unroll
-    for (int e = 0; e < N; ++e) o[r][e] = across<LPR>(o[r][e] * w, add);
-    if (lane < LPR)
+    for (int r = 0; r < NR; ++r) {
 #pragma unroll
-      for (int e = 0; e < N; ++e) so[wave][r][d0 + e] = o[r][e];
-    if (lane == 0) {
-      sm[wave][r][0] = m[r];
-      sm[wave][r][1] = l[r];
+      for (int e = 0; e < N; ++e) {
+        o[r][e] = across<LPR>(o[r][e] * w[r], add);
+        if (lane < LPR) so[wave][r][d0 + e] = o[r][e];
+      }
+      if (lane == lane_of<NR>(r)) {
+        sm[wave][r][0] = top * a.c;
+        sm[wave][r][1] = l;
+      }
     }
   }
   __syncthreads();

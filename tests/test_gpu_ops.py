@@ -171,8 +171,12 @@ def test_cross_attention_masked_keys_touch_nothing(device, dtype, Lq):
     assert torch.equal(out, out2) and all(torch.equal(a, b) for a, b in zip(grads, grads2))
     assert not out[2].any() and not grads[0][2].any()
     assert not grads[1][~keep].any() and not grads[2][~keep].any()
+    # float16 without gradients is another kernel than with them (sums of float32 in another order, at
+    # the edge of a rounding another half), so the masks' types are compared within the one
+    alone = ops.cross_attention(q, k2, v2, keep, 0.2)
+    assert dtype == F16 or torch.equal(alone, out2)
     for mask in (keep.float(), keep.long() * 3, keep.to(torch.bfloat16)):
-        assert torch.equal(ops.cross_attention(q, k2, v2, mask, 0.2), out2)
+        assert torch.equal(ops.cross_attention(q, k2, v2, mask, 0.2), alone)
     one = keep[1:2]
     R.check(ops.cross_attention(q, k, v, one, 0.2), *R.attention(q, k, v, one, 0.2)["out"])
 
