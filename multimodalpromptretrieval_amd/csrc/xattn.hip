@@ -683,9 +683,10 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // LPR keys at a time; each such group of lanes keeps its own running maximum, sum and output share
 // of every row (the maximum moves as the tiled kernel's does), and they are joined when the keys are done.  The wave's next FEW_AHEAD reads are on
 // their way while the present ones are computed.  32 x 8 key heads of 4 rows, 8192 keys, D = 128 in
-// bf16: 199 us, 5.4 TB/s; 16 x 12 heads, 562 keys, D = 64 in fp32 9.6 us, half of it until the first
-// keys are there.  (Reading the first keys before the mask is known made masked batches slower, 66 us
-// against 60; blocks of 4 waves 207 us against 199.)
+// bf16: 190 us, 5.7 TB/s (with every lane taking every row's exponential 199, and 184 against 163 for
+// ragged lengths, where the longest head's blocks are bound by their vector work); 16 x 12 heads, 562
+// keys, D = 64 in fp32 9.6 us, half of it until the first keys are there.  (Reading the first keys
+// before the mask is known made masked batches slower, 66 us against 60.)
 constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
 
 template <int CTRL>
@@ -1332,8 +1333,8 @@ XPlan xattn_plan(const int64_t* dims) {
   p.few = R <= FEW_ROWS;
   if (p.few) {
     // One or two rows: two blocks a CU hide each other's beginning and end (160 heads of 4096 keys,
-    // D = 128 bf16: 43 us, with one a CU 48).  More rows keep the vector units busier than memory,
-    // and more shares only cost their joins (64 heads of 8192 keys, 4 rows: 52 us, with two 58).
+    // D = 128 bf16: 42 us, with one a CU 46).  More rows keep the vector units about as busy as memory,
+    // and more shares only cost their joins (64 heads of 8192 keys, 4 rows: 43 us, with two 49).
     p.fwd = tiling(heads, 1, Lk, R <= 2 ? 512 : 256, 512, 64);
     p.fwd.tiles = 1;
   } else {
