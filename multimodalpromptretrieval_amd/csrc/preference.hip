@@ -10,6 +10,7 @@
 // digits.  A label >= V gives NaN.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops.h"
 
@@ -45,25 +46,48 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
   return {m, a.s * exp_from(a.m, m) + b.s * exp_from(b.m, m)};
 }
 
-// stat[row * split + part] = the maximum and sum over the part's columns.  Bound by the read of the
+// what a stats launch leaves: per part of a row, or per row in one part
+union LpStat {
+  MaxSum* part;
+  double* lp;
+};
+// log softmax at a value v of a row, the terms in fp32, their difference in 64 bits
+__device__ __forceinline__ double lp_row(float v, MaxSum c) {
+  return (double)(v - c.m) - (double)logf(c.s);
+}
+
+// stat[row * split + part] = the maximum and sum over the part's columns; where a row is one part, what
+// becomes of them: row_stat and the label's log-probability (0 where it is ignored).  Bound by the read of the
 // labelled rows: 8192 rows of 32128 in bf16, five eighths of them labelled (329 MB), 48 us, 6.9 TB/s
 // (part of them from the caches); 320 rows of 32101 in fp32 6.4 us.
 template <class T>
 __global__ __launch_bounds__(LP_THREADS) void lp_stats_kernel(const T* __restrict__ x, LpArgs a,
-                                                              MaxSum* __restrict__ stat) {
+                                                              LpStat stat,
+                                                              MaxSum* __restrict__ row_stat) {
   constexpr int N = VEC16<T>, U = 4;
   __shared__ MaxSum red[LP_THREADS / 64];
   const int64_t row = blockIdx.x, s = row / a.T, t = row % a.T;
-  if (lp_label(a, s, t) < 0) return;
+  const int64_t y = lp_label(a, s, t);
+  if (y < 0) {
+    if (a.split == 1 && threadIdx.x == 0) stat.lp[row] = 0.0;
+    return;
+  }
   const T* xr = x + s * a.xs + t * a.xt;
+  const float at_label = y < a.V ? to_f<T>(xr[y]) : NAN;
   const int64_t nv = a.V / N, per = cdiv(nv, a.split);
   const int64_t lo = blockIdx.y * per, hi = min(nv, lo + per);
   MaxSum c = {-INFINITY, 0.f};
   int64_t i = lo + threadIdx.x;
-  for (; i + (U - 1) * LP_THREADS < hi; i += U * LP_THREADS) {
+  const auto step = [&](auto whole) {  // U accesses at once; not whole: those that there are
     float v[U][N];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_f<T, N>(xr + (i + u * LP_THREADS) * N, v[u]);
+    for (int u = 0; u < U; ++u) {
+      if (decltype(whole)::value || i + u * LP_THREADS < hi)
+        load_f<T, N>(xr + (i + u * LP_THREADS) * N, v[u]);
+      else
+#pragma unroll
+        for (int e = 0; e < N; ++e) v[u][e] = -INFINITY;
+    }
     float m = c.m;
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -75,18 +99,9 @@ __global__ __launch_bounds__(LP_THREADS) void lp_stats_kernel(const T* __restric
 #pragma unroll
       for (int e = 0; e < N; ++e) sum += exp_from(v[u][e], m);
     c = {m, sum};
-  }
-  for (; i < hi; i += LP_THREADS) {
-    float v[N];
-    load_f<T, N>(xr + i * N, v);
-    float m = c.m;
-#pragma unroll
-    for (int e = 0; e < N; ++e) m = fmaxf(m, v[e]);
-    float sum = c.s * exp_from(c.m, m);
-#pragma unroll
-    for (int e = 0; e < N; ++e) sum += exp_from(v[e], m);
-    c = {m, sum};
-  }
+  };
+  for (; i + (U - 1) * LP_THREADS < hi; i += U * LP_THREADS) step(std::true_type{});
+  if (i < hi) step(std::false_type{});
   if (blockIdx.y == gridDim.y - 1)
     for (int64_t j = nv * N + threadIdx.x; j < a.V; j += LP_THREADS) {
       const float v = to_f<T>(xr[j]), m = fmaxf(c.m, v);
@@ -99,37 +114,51 @@ __global__ __launch_bounds__(LP_THREADS) void lp_stats_kernel(const T* __restric
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < LP_THREADS / 64; ++w) c = join(c, red[w]);
-    stat[row * a.split + blockIdx.y] = c;
+    if (a.split == 1) {
+      row_stat[row] = {c.m, 1.f / c.s};
+      stat.lp[row] = lp_row(at_label, c);
+    } else {
+      stat.part[row * a.split + blockIdx.y] = c;
+    }
   }
 }
 
-// lp_s in 64 bits by one wave; row_stat[row] = (m, 1 / sum) for the backward
+// A thread's share of lp_s in 64 bits, of positions t0, t0 + step, ...; where rows are in parts,
+// row_stat[row] = (m, 1 / sum) for the backward
 template <class T>
-__device__ double lp_sequence(const T* x, const LpArgs& a, const MaxSum* stat, MaxSum* row_stat,
-                              int64_t s, int lane) {
+__device__ double lp_share(const T* x, const LpArgs& a, const LpStat& stat, MaxSum* row_stat,
+                           int64_t s, int t0, int step) {
   double lp = 0.0;
-  for (int64_t t = lane; t < a.T; t += 64) {
+  if (a.split == 1) {
+#pragma unroll 8
+    for (int64_t t = t0; t < a.T; t += step) lp += stat.lp[s * a.T + t];
+    return lp;
+  }
+  for (int64_t t = t0; t < a.T; t += step) {
     const int64_t y = lp_label(a, s, t);
     if (y < 0) continue;
     const int64_t row = s * a.T + t;
-    MaxSum c = stat[row * a.split];
-    for (int i = 1; i < a.split; ++i) c = join(c, stat[row * a.split + i]);
-    row_stat[row] = {c.m, 1.f / c.s};
     const float v = y < a.V ? to_f<T>(x[s * a.xs + t * a.xt + y]) : NAN;
-    lp += (double)(v - c.m) - (double)logf(c.s);
+    MaxSum c = stat.part[row * a.split];
+    for (int i = 1; i < a.split; ++i) c = join(c, stat.part[row * a.split + i]);
+    row_stat[row] = {c.m, 1.f / c.s};
+    lp += lp_row(v, c);
   }
-  return wave_add(lp);
+  return lp;
 }
 
+// lp_s, a block for each
 template <class T>
-__global__ __launch_bounds__(256) void lp_sequence_kernel(const T* x, LpArgs a, const MaxSum* stat,
+__global__ __launch_bounds__(256) void lp_sequence_kernel(const T* x, LpArgs a, LpStat stat,
                                                           MaxSum* row_stat, float* logps,
                                                           double* logps64) {
-  const int lane = threadIdx.x & 63;
-  const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (s >= a.S) return;
-  const double lp = lp_sequence(x, a, stat, row_stat, s, lane);
-  if (lane == 0) {
+  __shared__ double red[4];
+  const int64_t s = blockIdx.x;
+  const double part = wave_add(lp_share(x, a, stat, row_stat, s, threadIdx.x, 256));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = part;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const double lp = (red[0] + red[1]) + (red[2] + red[3]);
     logps[s] = (float)lp;
     logps64[s] = lp;
   }
@@ -164,18 +193,19 @@ __global__ __launch_bounds__(1024) void lp_pairs_kernel(const double* lp, const 
   lp_pairs(lp, ref, P, beta, eps, loss, dlp);
 }
 
-// Few sequences: both in one launch, a wave for each sequence in turn (16 sequences of 20: 5 us, and a
-// launch of 3.4 us of host time less).
+// Few sequences of few positions: both in one launch, a wave for each sequence in turn (16 sequences of
+// 20: 5 us, and a launch of 3.4 us of host time less).
 constexpr int LP_FEW = 64;
+constexpr int64_t LP_FEW_ROWS = 16384;
 template <class T>
-__global__ __launch_bounds__(1024) void lp_few_kernel(const T* x, LpArgs a, const MaxSum* stat,
+__global__ __launch_bounds__(1024) void lp_few_kernel(const T* x, LpArgs a, LpStat stat,
                                                       MaxSum* row_stat, float* logps,
                                                       const float* ref, double beta, double eps,
                                                       float* loss, float* dlp) {
   __shared__ double lp64[LP_FEW];
   const int lane = threadIdx.x & 63;
   for (int s = threadIdx.x >> 6; s < a.S; s += 16) {
-    const double lp = lp_sequence(x, a, stat, row_stat, s, lane);
+    const double lp = wave_add(lp_share(x, a, stat, row_stat, s, lane, 64));
     if (lane == 0) {
       logps[s] = (float)lp;
       lp64[s] = lp;
@@ -292,28 +322,31 @@ int mpr_logps_fwd(const void* logits, int32_t dtype, int64_t S, int64_t T, int64
                 (long long)ws_bytes, (long long)p.bytes);
     hipStream_t s = op_stream(stream);
     char* w = static_cast<char*>(ws);
-    MaxSum* stat = reinterpret_cast<MaxSum*>(w + p.stat);
+    LpStat stat;
+    stat.part = reinterpret_cast<MaxSum*>(w + p.stat);
+    const bool few = loss && S <= LP_FEW && p.rows <= LP_FEW_ROWS;
     double* lp64 = reinterpret_cast<double*>(w + p.lp64);
     const LpArgs a{labels, labels64, ls, xs, xt, S, T, V, p.split};
     MPR_TRY(by_dtype(dtype, [&](auto z) -> int {
       using X = decltype(z);
       const X* x = static_cast<const X*>(logits);
       if (p.rows) {
-        lp_stats_kernel<X><<<dim3((unsigned)p.rows, p.split), LP_THREADS, 0, s>>>(x, a, stat);
+        lp_stats_kernel<X><<<dim3((unsigned)p.rows, p.split), LP_THREADS, 0, s>>>(
+            x, a, stat, reinterpret_cast<MaxSum*>(row_stat));
         MPR_LAUNCHED();
       }
-      if (loss && S <= LP_FEW) {
+      if (few) {
         lp_few_kernel<X><<<1, 1024, 0, s>>>(x, a, stat, reinterpret_cast<MaxSum*>(row_stat), logps,
                                             ref, beta, label_smoothing, loss, dlogps);
         MPR_LAUNCHED();
         return MPR_OK;
       }
-      lp_sequence_kernel<X><<<dim3((unsigned)cdiv(S, 4)), 256, 0, s>>>(
+      lp_sequence_kernel<X><<<dim3((unsigned)S), 256, 0, s>>>(
           x, a, stat, reinterpret_cast<MaxSum*>(row_stat), logps, lp64);
       MPR_LAUNCHED();
       return MPR_OK;
     }));
-    if (!loss || S <= LP_FEW) return MPR_OK;
+    if (!loss || few) return MPR_OK;
     lp_pairs_kernel<<<1, 1024, 0, s>>>(lp64, ref, S / 2, beta, label_smoothing, loss, dlogps);
     MPR_LAUNCHED();
     return MPR_OK;
