@@ -248,9 +248,11 @@ __device__ __forceinline__ float halves(float x, F f) {
 // ---- staging -------------------------------------------------------------------------------------
 // A tile of ROWS rows from memory straight to LDS (no registers in between): starts the reads; they
 // have landed after landed() and a barrier.  A wave's call writes 64 neighbouring pieces, so the
-// permutation of a row's pieces is in what each lane reads.  Rows past `last` read that row and
-// pieces past column D the row's first: what they hold meets only zeros (patch(), or the register
-// operand's own zero columns).  at(r): the row's first element.
+// permutation of a row's pieces is in what each lane reads.  Rows past `last` read that row: what they
+// hold meets only zeros (patch()) or masked scores.  Pieces past column D read `zeros` (another piece
+// of the row would not do: an infinity there times the other operand's zero is NaN).  at(r): the
+// row's first element.
+__device__ const f32x4 zeros = {0.f, 0.f, 0.f, 0.f};
 template <class E, int DP, int ROWS, class At>
 __device__ __forceinline__ void stage(E* lds, int64_t r0, int64_t last, int D, At at, int wave,
                                       int lane) {
@@ -259,10 +261,11 @@ __device__ __forceinline__ void stage(E* lds, int64_t r0, int64_t last, int D, A
 #pragma unroll
   for (int i = 0; i < CNT; ++i) {
     const int first = (i * NW + wave) * 64, slot = first + lane, r = slot / CH;
-    int c = ((slot % CH) ^ swz(r)) * N;
-    c = c < D ? c : 0;
+    const int c = ((slot % CH) ^ swz(r)) * N;
+    const E* from = at(min(r0 + r, last)) + c;
+    from = c < D ? from : reinterpret_cast<const E*>(&zeros);
     __builtin_amdgcn_global_load_lds(
-        (const __attribute__((address_space(1))) void*)(at(min(r0 + r, last)) + c),
+        (const __attribute__((address_space(1))) void*)from,
         (__attribute__((address_space(3))) void*)(lds + first * N), 16, 0, 0);
   }
 }

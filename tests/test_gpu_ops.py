@@ -192,6 +192,23 @@ def test_cross_attention_nan_shows(device):
         assert torch.isfinite(out[0]).all() and torch.isfinite(out[1, :, 0]).all()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("D", [40, 64, 72])
+@pytest.mark.parametrize("Lq", [1, 40])
+def test_cross_attention_keys_of_minus_infinity(device, dtype, D, Lq):
+    """A key whose score is -inf has weight 0, whatever the tile pads the head with."""
+    g = gen(14)
+    q, k, v, _ = xattn_inputs(g, 2, 2, 2, Lq, 150, D, dtype)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    bad = torch.rand(2, 150, generator=g, device="cuda") < 0.3
+    k[bad] = k[bad].index_fill(-1, torch.tensor([0], device="cuda"), float("-inf"))
+    for keep in (None, torch.rand(2, 150, generator=g, device="cuda") < 0.8):
+        left = ~bad if keep is None else keep & ~bad
+        finite = torch.where(left[..., None, None], k, torch.zeros_like(k))
+        ref = R.attention(q, finite, v, left, 0.3, torch.zeros_like(q))
+        R.check(ops.cross_attention(q, k, v, keep, 0.3), *ref["out"])
+
+
 def test_cross_attention_empty(device):
     g = gen(9)
     for B, Lq, Lk in ((0, 3, 5), (2, 0, 5), (2, 3, 0)):
