@@ -1309,13 +1309,25 @@ constexpr int FEW_ROWS = 8;  // rows of a key head that the single-token kernel 
 struct Tiling {
   int nw = 1, tiles = 1, splits = 1, per = 0;
 };
-Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t least, int unit) {
+// fp32 blocks are bound by the matrix cores from start to end, so what counts is how many a CU gets:
+// as many shares as leave each of the `want` CUs one block, or three where that is two blocks of a
+// third each.  (8 x 8 heads, 256 x 1024, D = 64: 59 us and 147 us backward against 82 and 191 in one
+// share; a block of under 512 keys a wave does not pay for the join.  A bf16 block is shorter by
+// far and overlaps with others on its CU: the same in bf16 27 us against 22.)
+Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t least, int unit,
+              bool fp32 = false) {
   Tiling t;
   t.nw = n <= 32 ? 1 : n <= 64 ? 2 : NW;
   t.tiles = (int)std::max<int64_t>(1, cdiv(n, 32 * t.nw));
   const int64_t blocks = std::max<int64_t>(1, heads * t.tiles);
   int64_t s = 2 * blocks >= want ? 1 : cdiv(want, blocks);
+  if (fp32) {
+    s = std::max<int64_t>(1, want / blocks);
+    if (s == 1 && 3 * blocks <= 2 * want) s = 3;
+    if (2 * blocks >= want && other * t.nw < 512 * NW) s = 1;
+  }
   s = std::max<int64_t>(1, std::min(s, other / least));
+  if (fp32 && cdiv(blocks * s, want) >= s) s = 1;  // no fewer keys for a CU than in one share
   t.per = (int)(cdiv(cdiv(std::max<int64_t>(other, 1), s), unit) * unit);
   t.splits = (int)std::max<int64_t>(1, cdiv(other, t.per));
   return t;
@@ -1329,7 +1341,8 @@ struct XPlan {
 
 int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-XPlan xattn_plan(const int64_t* dims) {
+XPlan xattn_plan(const int64_t* dims, int32_t dtype) {
+  const bool fp32 = dtype == MPR_F32;
   const int64_t B = dims[0], H = dims[1], Hkv = dims[2], Lq = dims[3], Lk = dims[4], D = dims[5];
   const int64_t heads = B * Hkv, R = H / Hkv * Lq;
   XPlan p;
@@ -1341,10 +1354,10 @@ XPlan xattn_plan(const int64_t* dims) {
     p.fwd = tiling(heads, 1, Lk, R <= 2 ? 512 : 256, 512, 64);
     p.fwd.tiles = 1;
   } else {
-    p.fwd = tiling(heads, R, Lk, 256, 256, 128);
+    p.fwd = tiling(heads, R, Lk, 256, 256, 128, fp32);
   }
-  p.dq = tiling(heads, R, Lk, 256, 256, 128);
-  p.dkv = tiling(heads, Lk, R, 256, 256, 128);
+  p.dq = tiling(heads, R, Lk, 256, 256, 128, fp32);
+  p.dkv = tiling(heads, Lk, R, 256, 256, 128, fp32);
   int64_t at = 0;
   if (p.fwd.splits > 1) at = up256(p.fwd.splits * heads * R * D * 4);
   p.part_ms = at;
@@ -1370,7 +1383,7 @@ int xattn_check(const char* what, const int64_t* dims, int32_t dtype) {
   MPR_REQUIRE(D >= 8 && D <= 128 && D % 8 == 0, "%s: head dim %lld (a multiple of 8 up to 128)",
               what, (long long)D);
   MPR_REQUIRE(H / Hkv * Lq <= most && B * Hkv <= most, "%s: too many rows", what);
-  const XPlan p = xattn_plan(dims);
+  const XPlan p = xattn_plan(dims, dtype);
   for (const Tiling& t : {p.fwd, p.dq, p.dkv})
     MPR_REQUIRE(B * Hkv <= MAX_GRID_X / ((int64_t)t.tiles * t.splits), "%s: too many blocks", what);
   return MPR_OK;
@@ -1520,7 +1533,7 @@ int mpr_xattn_workspace(const int64_t* dims, int32_t dtype, int64_t* fwd_bytes,
   return ops_call("xattn_workspace", [&]() -> int {
     MPR_TRY(xattn_check("xattn_workspace", dims, dtype));
     MPR_REQUIRE(fwd_bytes && bwd_bytes, "xattn_workspace: null pointer");
-    const XPlan p = xattn_plan(dims);
+    const XPlan p = xattn_plan(dims, dtype);
     *fwd_bytes = p.fwd_bytes;
     *bwd_bytes = p.bwd_bytes;
     return MPR_OK;
@@ -1535,7 +1548,7 @@ int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* ke
     MPR_REQUIRE(strides && scale >= 0.f, "xattn_fwd: no strides, or a scale below 0");
     if (dims[0] * dims[3] == 0) return MPR_OK;
     MPR_REQUIRE(q && out && (dims[4] == 0 || (k && v)), "xattn_fwd: null pointer");
-    const XPlan p = xattn_plan(dims);
+    const XPlan p = xattn_plan(dims, dtype);
     MPR_REQUIRE(p.fwd_bytes == 0 || (ws && ws_bytes >= p.fwd_bytes),
                 "xattn_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
                 (long long)p.fwd_bytes);
@@ -1567,7 +1580,7 @@ int mpr_xattn_bwd(const void* q, const void* k, const void* v, const uint8_t* ke
     MPR_REQUIRE(dims[3] == 0 || (q && out && lse && dout), "xattn_bwd: null pointer");
     MPR_REQUIRE(dims[4] == 0 || (k && v), "xattn_bwd: null pointer");
     MPR_REQUIRE(!dk == !dv, "xattn_bwd: dk and dv are wanted together");
-    const XPlan p = xattn_plan(dims);
+    const XPlan p = xattn_plan(dims, dtype);
     MPR_REQUIRE(p.bwd_bytes == 0 || (ws && ws_bytes >= p.bwd_bytes),
                 "xattn_bwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
                 (long long)p.bwd_bytes);
