@@ -46,6 +46,7 @@ struct XArgs {
   uint64_t lq_mul;   // r / Lq = r lq_mul >> lq_shift for r < 2^30
   int lq_shift;
   int tiles, splits, per_split;  // blocks along the tiled axis, and shares of the other one
+  int longest_first;  // the batch entries in the order of their lengths
   float c;           // scale log2(e), above 0
   float slack;       // how far scores may pass the running maximum: 8 / c
   float scale;
@@ -411,6 +412,38 @@ __device__ __forceinline__ Job job_of(const XArgs& a) {
   return j;
 }
 
+// The same with the longest batch entries first, where their masks tell them apart: blocks that begin
+// together should take equally long, and the last ones to begin be short.  16 samples of a mask are
+// enough to order by, and any order gives the same results.  (8 x 12 heads, 997 x 2011 keys, lengths
+// of a quarter to all of them, D = 64 bf16: 55, 63 and 67 us in three orders given, 48, 51 and 62 so; 32 x
+// 12 heads, 512 x 2011 115 and 101; D = 128 the same either way.)
+constexpr int ORDER_MOST = 64, ORDER_SAMPLES = 16;
+__device__ __forceinline__ Job job_longest_first(const XArgs& a, int t) {
+  Job j = job_of(a);
+  if (!a.longest_first) return j;
+  __shared__ int kept[ORDER_MOST], chosen;
+  constexpr int AT_ONCE = 64 * NW / ORDER_SAMPLES;
+  const int sample = t % ORDER_SAMPLES;
+  const int64_t key = (int64_t)a.Lk * (2 * sample + 1) / (2 * ORDER_SAMPLES);
+#pragma unroll
+  for (int i = 0; i < ORDER_MOST / AT_ONCE; ++i) {
+    const int b = i * AT_ONCE + t / ORDER_SAMPLES;
+    const uint64_t on = __ballot(b < a.B && a.keep[b * a.keep_bs + key]);
+    if (sample == 0)
+      kept[b] = __popc((uint32_t)(on >> (t & 63 & ~(ORDER_SAMPLES - 1))) & ((1u << ORDER_SAMPLES) - 1));
+  }
+  __syncthreads();
+  if (t < a.B) {
+    int before = 0;
+    for (int b = 0; b < a.B; ++b) before += kept[b] > kept[t] || (kept[b] == kept[t] && b < t);
+    if (before == j.b) chosen = t;
+  }
+  __syncthreads();
+  j.b = chosen;
+  j.bh = (int64_t)j.b * a.Hkv + j.hk;
+  return j;
+}
+
 // The block's waves: WR of them along the rows (32 each), NW / WR along the staged keys, KT at a time.
 // OCC: waves a SIMD is to hold, which is what its registers are shared by.  Tiles are staged into one
 // buffer while the other is computed, where two fit.
@@ -517,7 +550,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
   __shared__ uint32_t words[SPAN / 32];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
-  const Job j = job_of(a);
+  const Job j = job_longest_first(a, t);
   const int row = (j.tile * WR + wr) * 32 + (lane & 31);
   const bool in = row < a.R;
   const RowAt ra = row_at(a, j.hk, in ? row : 0);
@@ -1009,7 +1042,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq
   __shared__ uint32_t words[SPAN / 32];
   const int t = threadIdx.x, lane = t & 63;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
-  const Job j = job_of(a);
+  const Job j = job_longest_first(a, t);
   const int row = (j.tile * WR + wr) * 32 + (lane & 31);
   const bool in = row < a.R;
   const RowAt ra = row_at(a, j.hk, in ? row : 0);
@@ -1415,7 +1448,9 @@ unsigned xattn_tile(XArgs& a, const Tiling& t) {
   a.tiles = t.tiles;
   a.splits = t.splits;
   a.per_split = t.per;
-  return (unsigned)((int64_t)a.B * a.Hkv * t.tiles * t.splits);
+  const int64_t blocks = (int64_t)a.B * a.Hkv * t.tiles * t.splits;
+  a.longest_first = a.keep && a.B > 1 && a.B <= ORDER_MOST && a.Lk >= 512 && blocks > 256;
+  return (unsigned)blocks;
 }
 
 // Storage type -> matrix core.

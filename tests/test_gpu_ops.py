@@ -234,6 +234,24 @@ def test_cross_attention_strides(device, dtype):
     xattn_check(q[:, :1], k, v, keep, 0.3, dout[:, :1])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+def test_cross_attention_ragged_batch(device, dtype):
+    """Entries of every length, an empty one among them, in more blocks than there are CUs: each gets
+    the same bits wherever it stands in the batch."""
+    g = gen(15)
+    B, H, Lq, Lk, D = 6, 8, 700, 600, 64
+    q, k, v, dout = xattn_inputs(g, B, H, H, Lq, Lk, D, dtype)
+    lens = torch.tensor([250, 600, 0, 31, 600, 480], device="cuda")
+    keep = torch.arange(Lk, device="cuda")[None] < lens[:, None]
+    out, grads = xattn_check(q, k, v, keep, 0.2, dout)
+    for order in ([5, 4, 3, 2, 1, 0], [2, 3, 0, 5, 1, 4]):
+        leaves = [t[order].requires_grad_() for t in (q, k, v)]
+        again = ops.cross_attention(*leaves, keep[order], 0.2)
+        assert torch.equal(again, out[order])
+        for x, y in zip(torch.autograd.grad(again, leaves, dout[order]), grads):
+            assert torch.equal(x, y[order])
+
+
 @pytest.mark.parametrize("Lq", [1, 12])
 def test_cross_attention_odd_strides_of_single_dims(device, Lq):
     """A dimension of size 1 has whatever stride it came with; an odd one is nobody's address."""
