@@ -396,11 +396,14 @@ class _PreferenceLoss(torch.autograd.Function):
         logps, loss, kept = _logps_fwd(logits, labels, (ref, beta, smooth))
         ctx.save_for_backward(logits, labels, kept)
         ctx.mark_non_differentiable(logps)
+        ctx.set_materialize_grads(False)  # or torch fills zeros for logps in every backward
         return loss, logps
 
     @staticmethod
     @_first_order
     def backward(ctx, dloss, _):
+        if dloss is None:
+            return None, None, None, None, None
         logits, labels, kept = ctx.saved_tensors
         return _logps_bwd(logits, labels, kept, None, dloss), None, None, None, None
 

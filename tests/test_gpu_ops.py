@@ -406,6 +406,24 @@ def test_preference_long_margins(device):
     R.check(torch.autograd.grad(loss, x)[0], *want["dlogits"])
 
 
+def test_preference_loss_without_a_gradient(device):
+    """A function behind the loss that passes no gradient on: none arrives, not the loss's own."""
+    class Stop(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return x.clone()
+
+        @staticmethod
+        def backward(ctx, dx):
+            return None
+
+    logits, labels, ref = pref_inputs(gen(25), 2, 3, 50, F32)
+    x = logits.requires_grad_()
+    loss, _ = ops.preference_loss(x, labels, ref)
+    got, = torch.autograd.grad(Stop.apply(loss) + 0 * x.sum(), x)
+    assert not got.any()
+
+
 # ---- gradient clipping ---------------------------------------------------------------------------
 def clip_want(grads, max_norm, eps=1e-6):
     norm = torch.stack([g.double().square().sum() for g in grads]).sum().sqrt()
