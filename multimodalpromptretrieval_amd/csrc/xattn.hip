@@ -1344,13 +1344,23 @@ struct Tiling {
 };
 // fp32 blocks are bound by the matrix cores from start to end, so what counts is how many a CU gets:
 // as many shares as leave each of the `want` CUs one block, or three where that is two blocks of a
-// third each.  (8 x 8 heads, 256 x 1024, D = 64: 59 us and 147 us backward against 82 and 191 in one
-// share; a block of under 512 keys a wave does not pay for the join.  A bf16 block is shorter by
-// far and overlaps with others on its CU: the same in bf16 27 us against 22.)
+// third each.  (4 x 8 heads, 600 x 1500, D = 128: 153 us and 556 us backward against 209 and 626 in
+// one share; a block of under 512 keys a wave does not pay for the join.  A bf16 block is shorter by
+// far and overlaps with others on its CU: it loses by that.)
 Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t least, int unit,
               bool fp32 = false) {
   Tiling t;
   t.nw = n <= 32 ? 1 : n <= 64 ? 2 : NW;
+  // Fewer rows a block, and more waves along the other axis: where the shares of that axis would not
+  // make half the blocks wanted either (2 x 8 heads, 128 rows x 449, D = 128 fp32: 70 us with 128 rows a
+  // block, 30 with 32), or where half the rows just make them (8 x 8 heads, 256 x 1024, D = 64: fp32 48
+  // us against 58 in two shares, bf16 18 against 22).
+  while (t.nw > 1) {
+    const int64_t blocks = heads * cdiv(n, 32 * t.nw), halved = heads * cdiv(n, 16 * t.nw);
+    const bool scarce = 2 * blocks * std::max<int64_t>(1, other / least) < want;
+    if (!scarce && !(halved <= want && 10 * halved >= 6 * want)) break;
+    t.nw /= 2;
+  }
   t.tiles = (int)std::max<int64_t>(1, cdiv(n, 32 * t.nw));
   const int64_t blocks = std::max<int64_t>(1, heads * t.tiles);
   int64_t s = 2 * blocks >= want ? 1 : cdiv(want, blocks);

@@ -235,6 +235,25 @@ def test_cross_attention_strides(device, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,D", [
+    (8, 8, 8, 300, 300, 128),   # blocks of 128 rows, and of 128 keys
+    (17, 8, 8, 50, 50, 64),     # of 64
+    (17, 8, 8, 50, 50, 128),
+    (1, 8, 8, 700, 3000, 64),   # of 128 rows, in shares of the keys
+    (1, 8, 2, 700, 700, 64),
+    (1, 4, 4, 1900, 1300, 128),
+    (5, 8, 8, 1300, 40, 80),    # of 128 rows, and of 64 keys over shares of the rows
+])
+def test_cross_attention_tiles(device, dtype, B, H, Hkv, Lq, Lk, D):
+    g = gen(Lq + Lk + D)
+    q, k, v, dout = xattn_inputs(g, B, H, Hkv, Lq, Lk, D, dtype)
+    xattn_check(q, k, v, None, D ** -0.5, dout)
+    keep = torch.rand(B, Lk, generator=g, device="cuda") < 0.8
+    keep[B // 2:, Lk // 3:] = False
+    xattn_check(q, k, v, keep, 0.2, dout)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=NAMES.get)
 def test_cross_attention_ragged_batch(device, dtype):
     """Entries of every length, an empty one among them, in more blocks than there are CUs: each gets
     the same bits wherever it stands in the batch."""
