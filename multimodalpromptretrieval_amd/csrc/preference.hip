@@ -59,7 +59,7 @@ __device__ __forceinline__ double lp_row(float v, MaxSum c) {
 // stat[row * split + part] = the maximum and sum over the part's columns; where a row is one part, what
 // becomes of them: row_stat and the label's log-probability (0 where it is ignored).  Bound by the read of the
 // labelled rows: 8192 rows of 32128 in bf16, five eighths of them labelled (329 MB), 48 us, 6.9 TB/s
-// (part of them from the caches); 320 rows of 32101 in fp32 6.4 us.
+// (part of them from the caches); 320 rows of 32101 in fp32 7 us.
 template <class T>
 __global__ __launch_bounds__(LP_THREADS) void lp_stats_kernel(const T* __restrict__ x, LpArgs a,
                                                               LpStat stat,
