@@ -172,8 +172,10 @@ __device__ __forceinline__ void lp_pairs(const double* lp, const float* ref, int
   double sum = 0.0;
   for (int64_t p = threadIdx.x; p < P; p += 1024) {
     const double m = beta * ((lp[p] - lp[P + p]) - ((double)ref[p] - (double)ref[P + p]));
-    // -log sigmoid(m) = log(1 + exp(-|m|)) + max(-m, 0);  -log sigmoid(-m) is m more
-    sum += log1p(exp(-fabs(m))) + fmax(-m, 0.0) + eps * m;
+    // -log sigmoid(m) = log(1 + exp(-|m|)) + max(-m, 0);  -log sigmoid(-m) is m more.  An answer with
+    // a token that the model rules out has an infinite margin: the term of weight 0 is left out, and
+    // the two of a negative margin are one (0 inf and inf - inf would be NaN)
+    sum += log1p(exp(-fabs(m))) + (m > 0.0 ? (eps == 0.0 ? 0.0 : eps * m) : (eps - 1.0) * m);
     const double g = beta / (double)P * (eps - 1.0 / (1.0 + exp(m)));
     dlp[p] = (float)g;
     dlp[P + p] = (float)-g;

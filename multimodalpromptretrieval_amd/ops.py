@@ -430,7 +430,8 @@ def preference_loss(logits, labels, ref_logps, beta: float = 0.1, label_smoothin
     reference model's ``sequence_logps``, hold the chosen answers first, then the rejected ones in
     the same order.  ``margin_p = beta ((logps[p] - logps[P + p]) - (ref[p] - ref[P + p]))`` and
     ``loss = mean_p -(1 - label_smoothing) log sigmoid(margin_p) - label_smoothing log
-    sigmoid(-margin_p)``.  ``loss`` (a float32 scalar) is differentiable by ``logits``; ``logps``
+    sigmoid(-margin_p)``; the margin of an answer that the model rules out (a label's logit of -inf) is
+    infinite, and its term the limit.  ``loss`` (a float32 scalar) is differentiable by ``logits``; ``logps``
     [2P] (float32) is for the metrics and is not."""
     _logps_shapes(logits, labels, "preference_loss")
     S = logits.shape[0]

@@ -425,6 +425,40 @@ def test_preference_long_margins(device):
     R.check(torch.autograd.grad(loss, x)[0], *want["dlogits"])
 
 
+@pytest.mark.parametrize("smooth", [0.0, 0.1])
+@pytest.mark.parametrize("P", [3, 40])  # one launch for the sequences and the pairs, and two
+@pytest.mark.parametrize("chosen,rejected", [(0, 1), (1, 0), (1, 1)])
+def test_preference_of_answers_that_are_ruled_out(device, P, smooth, chosen, rejected):
+    """A rejected answer with a token of probability 0 has margin inf, a chosen one -inf: the loss of
+    such a pair is the limit (a weight of 0 times an infinite term is none), and its gradient is there:
+    beta / P times a constant, so only the softmax is off."""
+    beta = 0.2
+    logits, labels, ref = pref_inputs(gen(26), P, 6, 300, F32)
+    labels[:, 0] = torch.arange(2 * P, device="cuda") + 10  # every answer has a token
+    out = [0] * chosen + [P + 1] * rejected
+    for s in out:
+        logits[s, 0, labels[s, 0]] = float("-inf")
+    lp, b_lp = R.preference(logits, labels)["logps"]
+    m = beta * ((lp[:P] - lp[P:]) - (ref[:P].double() - ref[P:].double()))
+    fin = torch.isfinite(m)
+    assert int((~fin).sum()) == chosen + rejected and not torch.isnan(m).any()
+    sp = torch.nn.functional.softplus
+    pairs = (1 - smooth) * sp(-m) + (smooth * sp(m) if smooth else 0.0)
+    x = logits.detach().requires_grad_()
+    loss, logps = ops.preference_loss(x, labels, ref, beta, smooth)
+    R.check(logps, lp, b_lp, "logps")
+    both, share = torch.cat([fin, fin]), float(fin.sum()) / P  # the finite pairs alone
+    rest = R.preference(logits[both], labels[both], ref[both], beta, smooth, upstream=share)
+    b_loss = share * rest["loss"][1] + 2 * R.U * pairs.mean().abs()
+    R.check(loss, pairs.mean(), b_loss, "loss")
+    dx, = torch.autograd.grad(loss, x)
+    R.check(dx[both], *rest["dlogits"], "dlogits")
+    g = beta / P * (smooth - torch.sigmoid(-m))
+    dlp = torch.cat([g, -g])
+    R.check(dx[~both], *R.preference(logits[~both], labels[~both],
+                                     dlogps=dlp[~both])["dlogits"], "dlogits of the others")
+
+
 def test_preference_loss_without_a_gradient(device):
     """A function behind the loss that passes no gradient on: none arrives, not the loss's own."""
     class Stop(torch.autograd.Function):
