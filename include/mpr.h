@@ -433,7 +433,8 @@ int mpr_embed_bwd(const float* dY, int32_t d, const int32_t* uniq, const int32_t
  *   elements) = {q batch, position, head, k .., v .., keep batch, dout batch, position, head (bwd
  *   only)}.  out [B, Lq, H, D], rest as out (bfloat16: what rounding took off out; NULL: not kept),
  *   lse [B, H, Lq] (base-2 log of the rows' sums); rest and lse may be NULL in a forward alone; dq as out (NULL: not wanted), dk / dv [B, Lk, Hkv, D] (both or none), all
- *   contiguous.  Heads lie at multiples of 4 bytes.  float16: forward, H / Hkv Lq <= 8 only.  A row without a key: 0.
+ *   contiguous.  Heads lie at multiples of 4 bytes.  float16: forward, H / Hkv Lq <= 8 only.  A row
+ *   without a key: 0; one whose kept keys all score -inf: NaN.
  *   mpr_logps_fwd: logps[s] = sum over t with labels[s, t] >= 0 of log softmax(logits[s, t])[label]
  *   (logits [S, T, V] with strides xs, xt, 1; labels row stride ls; a label >= V gives NaN), and
  *   row_stat [S, T, 2] for the backward.  With loss: sequences p and S / 2 + p are the chosen and

@@ -18,7 +18,9 @@
 // cancel: the forward divides by the sum of the rounded P (its weights then add up to 1), and it
 // keeps what rounding takes off O for that row sum.
 //
-// Masked keys count for nothing whatever they hold (NaN, infinities): they are staged as zeros.
+// Masked keys count for nothing whatever they hold (NaN, infinities): they are staged as zeros.  A row
+// of kept keys that all score -inf has no softmax: its sum is 0 as that of a row without a key is, and
+// what tells them apart is whether a key was there (NONE_FINITE); O and the saved statistic are NaN.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -61,6 +63,17 @@ struct XArgs {
 };
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// In the place of a share's sum: it has keys, and every score is -inf.  (The share's maximum is -inf,
+// so beside others it weighs 0 like any other value.)
+constexpr float NONE_FINITE = -1.f;
+// what a row's sum l of 0 makes of its output and of its statistic
+__device__ __forceinline__ float inv_sum(float l, bool some) {
+  return l == 0.f ? (some ? NAN : 0.f) : 1.f / l;
+}
+__device__ __forceinline__ float lse_of(float m, float l, bool some) {
+  return l == 0.f ? (some ? NAN : -INFINITY) : m + log2f(l);
+}
 
 // ---- the two matrix cores ------------------------------------------------------------------------
 // LDS tiles hold rows of DP elements in 16-byte pieces; piece c of row r lies at piece c ^ swz(r):
@@ -564,9 +577,11 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
                       in, a.D, lane);
   f32x16 acc[DP / 32] = {};
   float m = -INFINITY, l = 0.f;  // of the unscaled scores
+  bool some = false;             // the block's share has a key
   const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
   for_tiles<T, M, DP, WR, false>(lds, lds1, words, keep, k_lo, k_hi, a.D, k_at, v_at, t, wave, lane,
                                  [&](const E* ks, const E* vs, const uint32_t* on) {
+      some = true;
       const int u0 = wk * NU;
       uint32_t bits[NU], any = 0, all = ~0u;
 #pragma unroll
@@ -642,18 +657,18 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
     });
     if (lane < 32) {
       a.part_ms[2 * at] = m * a.c;
-      a.part_ms[2 * at + 1] = l;
+      a.part_ms[2 * at + 1] = some && l == 0.f ? NONE_FINITE : l;
     }
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inv_sum(l, some);
   const int64_t at = (((int64_t)j.b * a.Lq + ra.i) * a.H + ra.h) * a.D;
   for_runs<DP>(acc, lane, [&](int d, const float (&x)[4]) {
     const float y[4] = {x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv};
     if (d < a.D) store_out<T, 4>(a, at + d, y);
   });
   if (lane < 32 && a.lse)
-    a.lse[((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m * a.c + log2f(l);
+    a.lse[((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i] = lse_of(m * a.c, l, some);
 }
 
 // The splits of a row: rescaled to their common maximum and summed in order.  A wave per row, whose
@@ -676,9 +691,11 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
   for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[2] = {0.f, 0.f};
+  bool some = false;
   for (int s0 = 0; s0 < a.splits; s0 += 64) {  // a lane per split, for its weight
     const int n = min(64, a.splits - s0);
     const f32x2 x = s0 == 0 ? first : lane < n ? ms[(s0 + lane) * rows + at] : none;
+    some = some || __ballot(x[1] == NONE_FINITE);
     const float w = exp2_fast(x[0] - base);
     l += wave_add(w * x[1]);
     for (int s = 0; s < n; s += AHEAD) {
@@ -701,7 +718,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
   const int64_t bh = at / a.R;
   const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv);
   const RowAt ra = row_at(a, hk, (int)(at % a.R));
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inv_sum(l, some);
   const int64_t to = (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
@@ -710,7 +727,7 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
     if (d < a.D) store_out<T, 1>(a, to + d, y);
   }
   if (lane == 0 && a.lse)
-    a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = l == 0.f ? -INFINITY : m + log2f(l);
+    a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = lse_of(m, l, some);
 }
 
 // ---- a few rows (single tokens) ------------------------------------------------------------------
@@ -863,6 +880,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
   typedef typename Vec<T, N>::type Run;
   Run q[NR];
   float o[NR][N], m = -INFINITY, l = 0.f;  // m, l: of the lane's row, unscaled scores
+  bool some = false;                       // the wave has had a key
 #pragma unroll
   for (int r = 0; r < NR; ++r) {
     q[r] = Run{};
@@ -901,6 +919,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
       }
     };
     const auto take = [&](const Ahead& x) {
+      some = true;
       float s[FEW_AHEAD], top = m;
 #pragma unroll
       for (int u = 0; u < FEW_AHEAD; ++u) {
@@ -966,7 +985,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
       }
       if (lane == lane_of<NR>(r)) {
         sm[wave][r][0] = top * a.c;
-        sm[wave][r][1] = l;
+        sm[wave][r][1] = some && l == 0.f ? NONE_FINITE : l;
       }
     }
   }
@@ -978,26 +997,27 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void xattn_few_kernel(XArgs a) {
     for (int w = 0; w < FEW_WAVES; ++w) top = fmaxf(top, sm[w][r][0]);
     const float zero = top == -INFINITY ? 0.f : top;
     float x = 0.f, sum = 0.f;
+    bool none_finite = false;
 #pragma unroll
     for (int w = 0; w < FEW_WAVES; ++w) {
       const float f = exp2_fast(sm[w][r][0] - zero);
       x += f * so[w][r][d];
       sum += f * sm[w][r][1];
+      none_finite = none_finite || sm[w][r][1] == NONE_FINITE;
     }
     if (a.splits > 1) {
       const int64_t at = ((int64_t)split * a.B * a.Hkv + bh) * a.R + r;
       a.part[at * a.D + d] = x;
       if (d == 0) {
         a.part_ms[2 * at] = top;
-        a.part_ms[2 * at + 1] = sum;
+        a.part_ms[2 * at + 1] = none_finite && sum == 0.f ? NONE_FINITE : sum;
       }
     } else {
       const RowAt ra = row_at(a, hk, r);
-      const float y[1] = {sum == 0.f ? 0.f : x / sum};
+      const float y[1] = {sum == 0.f ? (none_finite ? NAN : 0.f) : x / sum};
       store_out<T, 1>(a, (((int64_t)b * a.Lq + ra.i) * a.H + ra.h) * a.D + d, y);
       if (d == 0 && a.lse)
-        a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] =
-            sum == 0.f ? -INFINITY : top + log2f(sum);
+        a.lse[((int64_t)b * a.H + ra.h) * a.Lq + ra.i] = lse_of(top, sum, none_finite);
     }
   }
 }

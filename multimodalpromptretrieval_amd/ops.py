@@ -279,7 +279,8 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
     key head sum its query heads'.  D is a multiple of 8 up to 128.  ``scale`` 1 is T5's.
     ``key_mask`` [B, Lk] (or [1, Lk]): the keys that are not 0 / False are attended to; what a
     masked key holds (NaN, infinities) touches nothing and its gradient is 0, and a row whose keys
-    are all masked, or Lk = 0, gives 0.  Any strides will do (the halves of a joint k | v
+    are all masked, or Lk = 0, gives 0.  A row whose keys are there and all score -inf (keys that hold
+    infinities) has no softmax: it gives NaN.  Any strides will do (the halves of a joint k | v
     projection); heads are read in place where their elements are adjacent and they begin at
     multiples of 4 bytes, and copied otherwise.  float16 is computed in float32 except for single
     tokens (up to 8 rows of queries to a key head, without gradients)."""

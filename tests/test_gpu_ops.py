@@ -209,6 +209,36 @@ def test_cross_attention_keys_of_minus_infinity(device, dtype, D, Lq):
         R.check(ops.cross_attention(q, k, v, keep, 0.3), *ref["out"])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=NAMES.get)
+@pytest.mark.parametrize("Lq,Lk", [(1, 150), (1, 3000), (3, 700), (40, 150), (40, 3000), (300, 200)])
+def test_cross_attention_rows_of_minus_infinity(device, dtype, Lq, Lk):
+    """A row whose kept keys all score -inf has no softmax: NaN, as its gradients are, and not the 0 of a
+    row without a key.  Shares and tiles of such keys beside finite ones weigh nothing."""
+    g = gen(16)
+    B, H, Hkv, D = 4, 4, 2, 64
+    q, k, v, dout = xattn_inputs(g, B, H, Hkv, Lq, Lk, D, dtype)
+    k, v = k.contiguous(), v.contiguous()
+    q[..., 0] = q[..., 0].abs() + 0.5
+    keep = torch.rand(B, Lk, generator=g, device="cuda") < 0.8
+    keep[2] = False
+    bad = torch.zeros(B, Lk, dtype=torch.bool, device="cuda")
+    bad[0] = keep[0]          # every key of the entry
+    bad[1, :Lk // 2] = True   # whole tiles, and shares, of another
+    k[..., 0] = torch.where(bad[..., None], float("-inf"), k[..., 0])
+    finite = torch.where(bad[..., None, None], torch.zeros_like(k), k)
+    ref = R.attention(q, finite, v, keep & ~bad, 0.3, dout)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+    for out in (ops.cross_attention(q, k, v, keep, 0.3), ops.cross_attention(*leaves, keep, 0.3)):
+        assert bool(torch.isnan(out[0]).all())
+        R.check(out[1:], *(t[1:] for t in ref["out"]), "out")
+    grads = torch.autograd.grad(out, leaves, dout)
+    assert bool(torch.isnan(grads[0][0]).all())
+    for x in grads[1:]:
+        assert bool(torch.isnan(x[0][keep[0]]).all()) and not bool(x[0][~keep[0]].any())
+    for x, name in zip(grads, ("dq", "dk", "dv")):
+        R.check(x[2:], *(t[2:] for t in ref[name]), name)
+
+
 def test_cross_attention_empty(device):
     g = gen(9)
     for B, Lq, Lk in ((0, 3, 5), (2, 0, 5), (2, 3, 0)):
