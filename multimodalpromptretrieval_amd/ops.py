@@ -21,7 +21,8 @@ be the current device.  Workspaces come from torch's caching allocator in every 
 several streams and captured graphs share nothing; nothing waits for the GPU, so device tensors may
 be captured into a graph (token ids and labels on the host are uploaded: not inside a capture).
 Results are the same bits on every run.  What a call cannot take is refused with ``ValueError`` /
-``TypeError`` before anything is launched.  The gradients themselves are not differentiable again.
+``TypeError`` before anything is launched.  The gradients themselves are not differentiable again;
+forward-mode derivatives and ``torch.jit.trace`` are refused (``NotImplementedError``).
 
 Capturing a backward pass: torch ties a leaf's gradient accumulation to the stream of the first
 graph that reached it, so drop every loss of the same leaves that ran eagerly (``del loss``) before
@@ -36,6 +37,7 @@ from functools import lru_cache
 from operator import attrgetter, index
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -64,6 +66,16 @@ def _same(a, b, what: str) -> None:
         raise ValueError(f"{what}: tensors on {a.device} and {b.device}")
     if a.dtype != b.dtype:
         raise TypeError(f"{what}: {a.dtype} and {b.dtype}")
+
+
+def _eager(what: str, tensors) -> None:
+    """Refuses what a call would otherwise lose without a word: the tangents of forward-mode
+    derivatives (no operator has a formula for them), and in a trace the kernels themselves."""
+    if torch._C._get_tracing_state() is not None:
+        raise NotImplementedError(f"{what}: torch.jit.trace cannot record libmpr's kernels")
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivative")
 
 
 def _rows(t):
@@ -190,6 +202,7 @@ def embed(weight, ids, scale: float = 1.0, padding_idx: int = None):
             raise ValueError(f"embed: padding_idx {padding_idx} in a table of {V} rows")
         pad = padding_idx % V
     scale = float(scale)
+    _eager("embed", (weight,))
     ids = _tokens(ids, weight.device, "embed ids", V, 0)
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embed.apply(weight, ids, scale, pad)
@@ -310,6 +323,7 @@ def cross_attention(q, k, v, key_mask=None, scale: float = 1.0):
         if key_mask.dim() != 2 or key_mask.shape[0] not in (1, B) or key_mask.shape[1] != Lk:
             raise ValueError(f"cross_attention: key_mask {tuple(key_mask.shape)}, "
                              f"needed [{B}, {Lk}]")
+    _eager("cross_attention", (q, k, v))
     _on_gpu(q, "cross_attention")
     if scale < 0.0:  # the kernels' running maximum is of unscaled scores
         q, scale = -q, -scale
@@ -418,6 +432,7 @@ def sequence_logps(logits, labels):
     device gives NaN (on the host: IndexError).  Under ``no_grad`` this is the reference model's
     side of ``preference_loss``."""
     _logps_shapes(logits, labels, "sequence_logps")
+    _eager("sequence_logps", (logits,))
     labels = _label_ids(logits, labels, "sequence_logps")
     if logits.requires_grad and torch.is_grad_enabled():
         return _SequenceLogps.apply(logits, labels)
@@ -448,6 +463,7 @@ def preference_loss(logits, labels, ref_logps, beta: float = 0.1, label_smoothin
         raise ValueError(f"preference_loss: beta {beta}")
     if not 0.0 <= smooth <= 0.5:
         raise ValueError(f"preference_loss: label_smoothing {smooth} (0 to 0.5)")
+    _eager("preference_loss", (logits, ref_logps))
     labels = _label_ids(logits, labels, "preference_loss")
     ref = ref_logps.detach().to(torch.float32).contiguous()
     if logits.requires_grad and torch.is_grad_enabled():
@@ -530,6 +546,9 @@ def _clip(grads, out, max_norm, eps, what):
         if not (mine and theirs and theirs[1] == mine[1] and
                 counts == array("q", map(_T.numel, out))):
             theirs = (_check_outs(grads, out, what),)
+    _eager(what, grads)
+    if out is not None:
+        _eager(what, out)
     _on_gpu(grads[0], what)
     device = grads[0].device
     table = array("q", bytes(40 * n))  # n x {pointer, values, type, output pointer, its type}

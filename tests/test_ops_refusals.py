@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from multimodalpromptretrieval_amd import _lib, ops
 
@@ -225,3 +226,41 @@ def test_clip_one_tensor_is_not_its_rows():
         ops.clip_grads_(T(3, 4), 1.0, out=T(3, 4))
     with pytest.raises(ValueError, match="GPU"):
         ops.grad_norm(T(()))
+
+
+def calls():
+    """(name, call of one floating tensor) of every operator, on the host (where each ends refused)."""
+    ids, x = T(2, 3, dtype=torch.int64), T(4, 3, 7)
+    y, q = T(4, 3, dtype=torch.int64) - 100, T(2, 3, 4, 64)
+    return [("embed", T(5, 4), lambda t: ops.embed(t, ids)),
+            ("cross_attention", q, lambda t: ops.cross_attention(t, q, q)),
+            ("cross_attention", q, lambda t: ops.cross_attention(q, t, q, T(2, 3), -0.5)),
+            ("cross_attention", q, lambda t: ops.cross_attention(q, q, t)),
+            ("cross_attention", q.half(), lambda t: ops.cross_attention(q.half(), q.half(), t)),
+            ("sequence_logps", x, lambda t: ops.sequence_logps(t, y)),
+            ("preference_loss", x, lambda t: ops.preference_loss(t, y, T(4))),
+            ("preference_loss", T(4), lambda t: ops.preference_loss(x, y, t)),
+            ("grad_norm", T(5), lambda t: ops.grad_norm([T(3), t])),
+            ("clip_grads_", T(5), lambda t: ops.clip_grads_([t, T(3)], 1.0)),
+            ("clip_grads_", T(5), lambda t: ops.clip_grads_([T(5)], 1.0, out=[t]))]
+
+
+@pytest.mark.parametrize("leaf", [False, True])
+def test_forward_mode_derivatives_are_refused(leaf):
+    """No operator has a formula for a tangent: without a word it would count as zero."""
+    for name, x, call in calls():
+        with forward_ad.dual_level():
+            with pytest.raises(ValueError, match="GPU"):
+                call(x)  # a level is open, the tensors carry nothing
+            dual = forward_ad.make_dual(x.requires_grad_(leaf), torch.ones_like(x))
+            with pytest.raises(NotImplementedError, match=name + ".*forward"):
+                call(dual)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match=name):
+                call(dual)
+
+
+def test_traces_are_refused():
+    """A trace would keep the output's memory and leave out the kernel that fills it."""
+    for name, x, call in calls():
+        with pytest.raises(NotImplementedError, match=name + ".*trace"):
+            torch.jit.trace(call, x, check_trace=False)
