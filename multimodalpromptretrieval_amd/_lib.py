@@ -237,10 +237,19 @@ def exported_symbols() -> list:
     return [name for name, _, _ in SIGNATURES]
 
 
+MPR_EINVAL = -1
+
+
+class InvalidArgument(ValueError, RuntimeError):
+    """An argument that the library refuses (MPR_EINVAL): a ValueError, and like its other errors a
+    RuntimeError."""
+
+
 def check(rc: int, what: str = "") -> None:
     if rc != 0:
         msg = load().mpr_last_error()
-        raise RuntimeError(f"libmpr {what} failed ({rc}): {msg.decode() if msg else ''}")
+        error = InvalidArgument if rc == MPR_EINVAL else RuntimeError
+        raise error(f"libmpr {what} failed ({rc}): {msg.decode() if msg else ''}")
 
 
 def call(name: str, *args) -> int:

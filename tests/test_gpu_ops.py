@@ -593,6 +593,19 @@ def test_clip_layouts(device):
         ops.clip_grads_([a], 1.0, out=[torch.empty(50, 30, device="cuda")])
 
 
+def test_what_the_library_refuses_is_a_value_error(device):
+    g = gen(36)
+    flat = randn(g, 100)
+    with pytest.raises(ValueError, match="overlap"):
+        ops.clip_grads_([flat, flat], 1.0)
+    q, k = randn(g, 1, 1, 65537, 8), randn(g, 1, 3, 1, 8)
+    with pytest.raises(ValueError, match="65537 query heads"):
+        ops.cross_attention(q, k, k)
+    with pytest.raises(ValueError, match="positions"):
+        ops.sequence_logps(flat[:2].expand(1 << 12, 1 << 12, 2),
+                           torch.zeros((), dtype=torch.int64, device="cuda").expand(1 << 12, 1 << 12))
+
+
 def test_clip_one_tensor(device):
     """A tensor alone, its rows not being the list."""
     g = gen(34)

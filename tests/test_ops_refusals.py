@@ -264,3 +264,21 @@ def test_traces_are_refused():
     for name, x, call in calls():
         with pytest.raises(NotImplementedError, match=name + ".*trace"):
             torch.jit.trace(call, x, check_trace=False)
+
+
+def test_refusals_of_the_library_are_value_errors():
+    """What only the library knows to be too much is refused as the documentation says."""
+    n = ctypes.c_int64()
+    for name, *args in (("mpr_embed_grad_workspace", 0, 1 << 31, 5, 4, ctypes.byref(n)),
+                        ("mpr_xattn_workspace", i64(1, 65537, 1, 1, 1, 64), 0, ctypes.byref(n),
+                         ctypes.byref(n)),
+                        ("mpr_logps_workspace", 1 << 20, 1 << 20, 5, ctypes.byref(n)),
+                        ("mpr_clip_grads", 1, i64(4096, 4, 0, 4100, 0), 1.0, 0.0, P, P, 1 << 40,
+                         None)):
+        with pytest.raises(ValueError, match=name.replace("mpr_", "")):
+            _lib.call(name, *args)
+    st = (64, 64, 64, 1)
+    with pytest.raises(ValueError, match="65537 query heads"):
+        ops._xattn_plan(0, (1, 1, 65537, 64), (1, 1, 1, 64), st, st, st, 0, (0, 0, 0))
+    with pytest.raises(ValueError, match="sequences"):
+        ops._logps_plan(1 << 20, 1 << 20, 5)
