@@ -349,33 +349,35 @@ __device__ __forceinline__ void sum_flush(const SumArgs& a, T* dw, int64_t w, ui
 }
 
 // Blocks [0, zero_blocks): the rows of dW without a token become zero (a wave looks its rows up in
-// the sorted keys).  The others: a wave per window of `win` sorted positions and slab of 64
-// accesses of N columns, the rows' loads SUM_AHEAD ahead of their additions.  Bound by the reads of
-// dout: 262144 rows of 1024 in bf16, 30 % of them padding that is skipped (376 MB in, 66 MB out), 102 us,
-// 4.3 TB/s; 8992 rows of 768 in fp32 (28 MB in, 99 MB out) 19 us, 6.6 TB/s.
+// the sorted keys, ZERO_ROWS at a time).  The others: a wave per window of `win` sorted positions and
+// slab of 64 accesses of N columns, the rows' loads SUM_AHEAD ahead of their additions.  Bound by the
+// reads of dout: 262144 rows of 1024 in bf16, 30 % of them padding that is skipped (376 MB in, 66 MB
+// out), 102 us, 4.3 TB/s; 8992 rows of 768 in fp32 (28 MB in, 99 MB out) 19 us, 6.6 TB/s.
 template <class T, int N>
 __global__ __launch_bounds__(256) void embed_sum_kernel(const T* __restrict__ dout, SumArgs a,
                                                         T* __restrict__ dw) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   if (blockIdx.x < a.zero_blocks) {
-    const int64_t r0 = ((int64_t)blockIdx.x * 4 + wave) * ZERO_ROWS;
-    const int64_t row = r0 + lane;
-    bool empty = false;
-    if (lane < ZERO_ROWS && row < a.V) {
-      int64_t lo = 0, hi = a.n;  // the first sorted position with key >= row
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (a.key[mid] < (uint32_t)row) lo = mid + 1; else hi = mid;
+    for (int64_t r0 = ((int64_t)blockIdx.x * 4 + wave) * ZERO_ROWS; r0 < a.V;
+         r0 += a.zero_blocks * 4 * ZERO_ROWS) {
+      const int64_t row = r0 + lane;
+      bool empty = false;
+      if (lane < ZERO_ROWS && row < a.V) {
+        int64_t lo = 0, hi = a.n;  // the first sorted position with key >= row
+        while (lo < hi) {
+          const int64_t mid = (lo + hi) >> 1;
+          if (a.key[mid] < (uint32_t)row) lo = mid + 1; else hi = mid;
+        }
+        empty = lo == a.n || a.key[lo] != (uint32_t)row;
       }
-      empty = lo == a.n || a.key[lo] != (uint32_t)row;
-    }
-    const uint64_t todo = __ballot(empty);
-    for (int r = 0; r < ZERO_ROWS; ++r) {
-      if (!((todo >> r) & 1)) continue;
-      T* o = dw + (r0 + r) * a.d;
-      float z[N] = {};
-      for (int c = lane * N; c + N <= a.d; c += 64 * N) store_f<T, N>(o + c, z);
+      const uint64_t todo = __ballot(empty);
+      for (int r = 0; r < ZERO_ROWS; ++r) {
+        if (!((todo >> r) & 1)) continue;
+        T* o = dw + (r0 + r) * a.d;
+        float z[N] = {};
+        for (int c = lane * N; c + N <= a.d; c += 64 * N) store_f<T, N>(o + c, z);
+      }
     }
     return;
   }
@@ -499,6 +501,8 @@ int64_t align256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 // Window: the largest of 256 .. 8 positions that still gives SUM_WAVES waves (a longer window leaves
 // fewer partial sums of the runs that cross windows; fewer waves leave memory idle).
 constexpr int64_t SUM_WAVES = 4096;
+constexpr int64_t ZERO_BLOCKS = (int64_t)1 << 20;  // tables of more than 2^26 rows: several turns each
+constexpr int64_t SUM_GRID = ((int64_t)1 << 24) - 1;  // less than 2^32 threads in blocks of 256
 
 EmbedGrad embed_plan(int64_t n, int64_t V, int d, int vec) {
   EmbedGrad p;
@@ -528,10 +532,11 @@ int embed_vec(int32_t dtype, int d) {
   return d % v ? 1 : v;
 }
 
+int64_t sum_blocks(const SumArgs& a) { return a.zero_blocks + cdiv(a.wins * a.slabs, 4); }
+
 template <class T, int N>
 int embed_sums(const void* dout, const SumArgs& a, void* dw, hipStream_t s) {
-  const int64_t blocks = a.zero_blocks + cdiv(a.wins * a.slabs, 4);
-  MPR_REQUIRE(blocks <= MAX_GRID_X && a.wins <= MAX_GRID_X, "embed_grad: too many positions");
+  const int64_t blocks = sum_blocks(a);
   embed_sum_kernel<T, N><<<dim3((unsigned)blocks), 256, 0, s>>>(static_cast<const T*>(dout), a,
                                                                  static_cast<T*>(dw));
   MPR_LAUNCHED();
@@ -606,11 +611,13 @@ int mpr_embed_grad(const void* dout, int32_t dtype, int64_t ld, const void* ids,
     SumArgs a{};
     a.n = n; a.V = V; a.ld = ld; a.d = d; a.scale = scale;
     a.win = 1; a.slabs = 1;
-    a.zero_blocks = cdiv(V, 4 * ZERO_ROWS);
+    a.zero_blocks = std::min(cdiv(V, 4 * ZERO_ROWS), ZERO_BLOCKS);
     if (n) {
       p = embed_plan(n, V, d, vec);
       MPR_REQUIRE(ws && ws_bytes >= p.bytes, "embed_grad: workspace of %lld bytes, %lld needed",
                   (long long)ws_bytes, (long long)p.bytes);
+      a.win = p.win; a.wins = p.wins; a.slabs = p.slabs;
+      MPR_REQUIRE(sum_blocks(a) <= SUM_GRID && a.wins <= SUM_GRID, "embed_grad: too many positions");
       char* w = static_cast<char*>(ws);
       uint32_t* key[2] = {reinterpret_cast<uint32_t*>(w + p.key[0]),
                           reinterpret_cast<uint32_t*>(w + p.key[1])};
@@ -643,7 +650,6 @@ int mpr_embed_grad(const void* dout, int32_t dtype, int64_t ld, const void* ids,
         src.pos = pos[i & 1];
       }
       a.key = src.key; a.pos = src.pos;
-      a.win = p.win; a.wins = p.wins; a.slabs = p.slabs;
       a.head = reinterpret_cast<float*>(w + p.head);
       a.tail = reinterpret_cast<float*>(w + p.tail);
     }

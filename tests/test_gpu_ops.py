@@ -825,6 +825,22 @@ def test_embed_more_rows_than_a_launch_takes(device):
         assert torch.equal(got[part, 0], w[:, 0][ids[part].long()])
 
 
+def test_embed_gradient_of_more_rows_than_a_launch_takes(device):
+    V = (1 << 30) + 77  # 64 rows a block: more than 2^24 blocks
+    w = torch.ones(V, 1, device="cuda", dtype=BF16).requires_grad_()
+    ids = torch.tensor([5, V - 1, 5, 1 << 26, V - 2], device="cuda")
+    dout = randn(gen(106), 5, 1, dtype=BF16)
+    for n in (5, 0):
+        torch.ones_like(w)  # what the gradient's memory holds before
+        dw, = torch.autograd.grad(ops.embed(w, ids[:n]), w, dout[:n])
+        want = torch.zeros(3, 1, dtype=torch.float64, device="cuda") if n == 0 else torch.stack(
+            [dout[0].double() + dout[2].double(), dout[3].double(), dout[4].double()])
+        at = torch.tensor([5, 1 << 26, V - 2], device="cuda")
+        R.check(dw.detach()[at], want, 8 * R.U * want.abs() + R.rounded(want, BF16))
+        assert torch.equal(dw[V - 1], dout[1]) if n else not bool(dw[V - 1].any())
+        assert int(torch.count_nonzero(dw)) == (4 if n else 0)
+
+
 def test_cross_attention_past_32_bits(device):
     Lk, Hkv, D = (1 << 21) + 45, 8, 128  # Lk Hkv D > 2^31
     g = gen(102)

@@ -282,3 +282,9 @@ def test_refusals_of_the_library_are_value_errors():
         ops._xattn_plan(0, (1, 1, 65537, 64), (1, 1, 1, 64), st, st, st, 0, (0, 0, 0))
     with pytest.raises(ValueError, match="sequences"):
         ops._logps_plan(1 << 20, 1 << 20, 5)
+
+
+def test_embed_gradient_is_refused_before_its_sort():
+    with pytest.raises(ValueError, match="too many positions"):
+        _lib.call("mpr_embed_grad", P, 0, 1 << 21, P, 1, (1 << 31) - 1, 5, 1 << 21, 1.0, -1, P, P,
+                  1 << 62, None)
