@@ -445,7 +445,7 @@ int mpr_embed_bwd(const float* dY, int32_t d, const int32_t* uniq, const int32_t
  *   the label is ignored.
  *   mpr_clip_grads: desc = n x {pointer, values, dtype, output pointer, output dtype} (int64): norm
  *   = the L2 norm of all, output = value * min(1, max_norm / (norm + eps)).  The output may be the
- *   tensor itself; no output anywhere (0): the norm alone.  Memory that overlaps is refused. */
+ *   tensor itself; no output anywhere (0): the norm alone.  With outputs, memory that overlaps is refused. */
 int mpr_embed_lookup(const void* table, int32_t dtype, int64_t V, int64_t ld, const void* ids,
                      int32_t ids64, int64_t n, int32_t d, float scale, void* out, void* stream);
 int mpr_embed_grad_workspace(int32_t dtype, int64_t n, int64_t V, int32_t d, int64_t* bytes);

@@ -218,10 +218,10 @@ int64_t clip_chunks(const int64_t* desc, int n) {
   return c;
 }
 
-int clip_check(int n, const int64_t* desc) {
-  MPR_REQUIRE(n >= 0 && (n == 0 || desc), "clip_grads: %d tensors", n);
+// scale: outputs are wanted.  The norm alone reads, and what it reads may overlap.
+int clip_check(int n, const int64_t* desc, bool scale) {
   std::vector<Span> spans;
-  spans.reserve(2 * (size_t)n);
+  if (scale) spans.reserve(2 * (size_t)n);
   for (int i = 0; i < n; ++i) {
     const int64_t* d = desc + 5 * (int64_t)i;
     MPR_REQUIRE(d[1] >= 0 && d[1] <= (int64_t)1 << 37, "clip_grads: tensor %d has %lld values", i,
@@ -231,11 +231,13 @@ int clip_check(int n, const int64_t* desc) {
                 (long long)d[4]);
     if (d[1] == 0) continue;
     MPR_REQUIRE(d[0], "clip_grads: tensor %d is null", i);
+    if (!scale) continue;
+    MPR_REQUIRE(d[3], "clip_grads: tensor %d has no output", i);
     MPR_REQUIRE(d[3] != d[0] || d[4] == d[2],
                 "clip_grads: tensor %d is clipped in place into another type", i);
     const uintptr_t a = (uintptr_t)d[0], o = (uintptr_t)d[3];
     spans.push_back({a, a + (size_t)d[1] * (d[2] == MPR_F32 ? 4 : 2)});
-    if (o && o != a) spans.push_back({o, o + (size_t)d[1] * (d[4] == MPR_F32 ? 4 : 2)});
+    if (o != a) spans.push_back({o, o + (size_t)d[1] * (d[4] == MPR_F32 ? 4 : 2)});
   }
   std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
   for (size_t i = 1; i < spans.size(); ++i)
@@ -262,13 +264,11 @@ int mpr_clip_workspace(int32_t n, const int64_t* desc, int64_t* bytes) {
 int mpr_clip_grads(int32_t n, const int64_t* desc, double max_norm, double eps, float* norm,
                    void* ws, int64_t ws_bytes, void* stream) {
   return ops_call("clip_grads", [&]() -> int {
-    MPR_TRY(clip_check(n, desc));
-    MPR_REQUIRE(norm, "clip_grads: no place for the norm");
+    MPR_REQUIRE(n >= 0 && (n == 0 || desc), "clip_grads: %d tensors", n);
     bool scale = false;
     for (int i = 0; i < n; ++i) scale = scale || desc[5 * (int64_t)i + 3];
-    for (int i = 0; i < n; ++i)
-      MPR_REQUIRE(!scale || desc[5 * (int64_t)i + 1] == 0 || desc[5 * (int64_t)i + 3],
-                  "clip_grads: tensor %d has no output", i);
+    MPR_TRY(clip_check(n, desc, scale));
+    MPR_REQUIRE(norm, "clip_grads: no place for the norm");
     const int64_t chunks = clip_chunks(desc, n);
     MPR_REQUIRE(ws && ws_bytes >= (int64_t)sizeof(ClipState) + 8 * chunks,
                 "clip_grads: workspace of %lld bytes, %lld needed", (long long)ws_bytes,

@@ -571,7 +571,8 @@ def _clip(grads, out, max_norm, eps, what):
 @torch.no_grad()
 def grad_norm(grads):
     """The L2 norm of all values of the tensors (or the one tensor) together: a float32 scalar on their
-    device, 0 on the host for none.  Squares are summed in 64 bits."""
+    device, 0 on the host for none.  Squares are summed in 64 bits; a tensor listed twice counts
+    twice.  Tensors with gaps in their memory are refused."""
     return _clip(_listed(grads), None, None, 0.0, "grad_norm")
 
 

@@ -606,6 +606,18 @@ def test_what_the_library_refuses_is_a_value_error(device):
                            torch.zeros((), dtype=torch.int64, device="cuda").expand(1 << 12, 1 << 12))
 
 
+def test_norm_of_tensors_that_share_memory(device):
+    """The norm only reads: a tensor listed twice counts twice, overlapping parts each for itself."""
+    flat = randn(gen(37), 50000)
+    for some in ([flat, flat], [flat[:30000], flat[20000:], flat[5:6]]):
+        want, _ = clip_want(some, 1.0)
+        assert abs(float(ops.grad_norm(some)) - float(want)) <= 2 * R.U * float(want)
+        with pytest.raises(ValueError, match="overlap"):
+            ops.clip_grads_(some, 1.0)
+    with pytest.raises(ValueError, match="overlap"):  # read twice, but written next to it
+        ops.clip_grads_([flat, flat], 1.0, out=[torch.empty_like(flat), flat])
+
+
 def test_clip_one_tensor(device):
     """A tensor alone, its rows not being the list."""
     g = gen(34)
