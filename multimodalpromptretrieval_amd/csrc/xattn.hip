@@ -1396,6 +1396,42 @@ Tiling tiling(int64_t heads, int64_t n, int64_t other, int64_t want, int64_t lea
   return t;
 }
 
+// Shares of the keys for the single-token kernel, whose blocks (one a CU at a time) come in rounds of
+// CUS: the number whose rounds are over first.  A round takes as long as one block reads its keys, or,
+// with more blocks than memory serves at that rate (saturated: 176 of up to 4 rows, whose times at 64,
+// 128, 192 and 255 heads of 8192 keys, D = 128 bf16, are 140, 144, 162 and 205 us; 240 of more rows,
+// which the vector units bind), as long as memory takes; a block's beginning and end cost about as much
+// as reading 24 KB for each row (256 heads of 8 rows, 4096 keys: 117 us in one share, 130 in two, 151
+// in four), the join as 48 KB.  Measured with 4 rows, 8192 keys: 96 heads in 2 shares 94 us (in 1: 142,
+// in 3: 123), 128 in 2 112 (144), 160 in 3 136 (148; in 2: 176), 192 in 1 162 (in 2: 180), 320 in 4 259
+// (326); 8 rows, 4096 keys: 128 in 2 76 (109), 160 in 3 100 (111; in 2: 125).
+// Under a mask that reckoning does not hold (shares behind an entry's length end at once and even the
+// others out), so few heads are shared until each CU has a block, or two of one or two rows, as long as
+// that is more than one share: lengths of a quarter to all of 6144 keys, 4 rows, 88 heads in 3 61 us
+// (in 2, the best without a mask: 72); 1 row, 176 heads in 3 88 us (in 1: 106).
+constexpr int64_t CUS = 256, FEW_LEAST = 512;  // keys of a share
+Tiling few_tiling(int64_t heads, int64_t R, int64_t Lk, int64_t key_bytes, bool masked) {
+  const double saturated = R <= 4 ? 176 : 240, ends = 24576. * R / key_bytes;
+  const int64_t most = std::max<int64_t>(1, Lk / FEW_LEAST);
+  Tiling t;
+  double least = 0;
+  for (int rounds = 0; rounds <= 8; ++rounds) {  // the most shares of so many rounds; 0: one share
+    const int64_t s = std::min(most, std::max<int64_t>(1, rounds * CUS / std::max<int64_t>(1, heads)));
+    const int64_t blocks = heads * s, last = blocks % CUS;
+    const double each = blocks / CUS * (CUS / saturated) + (last ? std::max(1., last / saturated) : 0.);
+    const double time = each * ((double)cdiv(Lk, s) + ends) + (s > 1 ? 49152. / key_bytes : 0.);
+    if (rounds && time >= least) continue;
+    least = time;
+    t.splits = (int)s;
+  }
+  const int64_t want = R <= 2 ? 2 * CUS : CUS;
+  if (masked && 2 * heads < want)
+    t.splits = (int)std::min(most, cdiv(want, std::max<int64_t>(1, heads)));
+  t.per = (int)(cdiv(cdiv(std::max<int64_t>(Lk, 1), t.splits), 64) * 64);
+  t.splits = (int)std::max<int64_t>(1, cdiv(Lk, t.per));
+  return t;
+}
+
 struct XPlan {
   Tiling fwd, dq, dkv;
   bool few;
@@ -1404,27 +1440,25 @@ struct XPlan {
 
 int64_t up256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-XPlan xattn_plan(const int64_t* dims, int32_t dtype) {
+// (the forward's bytes are the most that either mask or none needs)
+XPlan xattn_plan(const int64_t* dims, int32_t dtype, bool masked = false) {
   const bool fp32 = dtype == MPR_F32;
   const int64_t B = dims[0], H = dims[1], Hkv = dims[2], Lq = dims[3], Lk = dims[4], D = dims[5];
   const int64_t heads = B * Hkv, R = H / Hkv * Lq;
   XPlan p;
   p.few = R <= FEW_ROWS;
-  if (p.few) {
-    // One or two rows: two blocks a CU hide each other's beginning and end (160 heads of 4096 keys,
-    // D = 128 bf16: 42 us, with one a CU 46).  More rows keep the vector units about as busy as memory,
-    // and more shares only cost their joins (64 heads of 8192 keys, 4 rows: 43 us, with two 49).
-    p.fwd = tiling(heads, 1, Lk, R <= 2 ? 512 : 256, 512, 64);
-    p.fwd.tiles = 1;
-  } else {
-    p.fwd = tiling(heads, R, Lk, 256, 256, 128, fp32);
-  }
+  const auto forward = [&](bool m) {
+    return p.few ? few_tiling(heads, R, Lk, 2 * D * (fp32 ? 4 : 2), m)
+                 : tiling(heads, R, Lk, 256, 256, 128, fp32);
+  };
+  p.fwd = forward(masked);
   p.dq = tiling(heads, R, Lk, 256, 256, 128, fp32);
   p.dkv = tiling(heads, Lk, R, 256, 256, 128, fp32);
+  const int64_t splits = std::max(p.fwd.splits, forward(!masked).splits);
   int64_t at = 0;
-  if (p.fwd.splits > 1) at = up256(p.fwd.splits * heads * R * D * 4);
+  if (splits > 1) at = up256(splits * heads * R * D * 4);
   p.part_ms = at;
-  p.fwd_bytes = at + (p.fwd.splits > 1 ? p.fwd.splits * heads * R * 8 : 0);
+  p.fwd_bytes = at + (splits > 1 ? splits * heads * R * 8 : 0);
   p.delta = 0;
   const int64_t base = up256(B * H * Lq * 4);
   int64_t part = p.dq.splits > 1 ? p.dq.splits * heads * R * D * 4 : 0;
@@ -1613,7 +1647,7 @@ int mpr_xattn_fwd(const void* q, const void* k, const void* v, const uint8_t* ke
     MPR_REQUIRE(strides && scale >= 0.f, "xattn_fwd: no strides, or a scale below 0");
     if (dims[0] * dims[3] == 0) return MPR_OK;
     MPR_REQUIRE(q && out && (dims[4] == 0 || (k && v)), "xattn_fwd: null pointer");
-    const XPlan p = xattn_plan(dims, dtype);
+    const XPlan p = xattn_plan(dims, dtype, keep != nullptr);
     MPR_REQUIRE(p.fwd_bytes == 0 || (ws && ws_bytes >= p.fwd_bytes),
                 "xattn_fwd: workspace of %lld bytes, %lld needed", (long long)ws_bytes,
                 (long long)p.fwd_bytes);

@@ -209,6 +209,32 @@ def test_workspaces_grow_with_the_work():
     assert bwd.value >= 4 * 16 * 1024 * 4
 
 
+def shares(B, H, Hkv, Lq, Lk, D, dtype):
+    """How many shares a forward's keys are in (with a mask or without, whichever are more), from its
+    workspace: a row of D floats and two more for each (the first part in whole 256 bytes); one share
+    needs none."""
+    fwd, bwd = ctypes.c_int64(), ctypes.c_int64()
+    _lib.call("mpr_xattn_workspace", i64(B, H, Hkv, Lq, Lk, D), dtype, ctypes.byref(fwd),
+              ctypes.byref(bwd))
+    return max(1, round(fwd.value / (B * H * Lq * (D + 2) * 4)))
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 8])
+@pytest.mark.parametrize("B,Hkv", [(1, 1), (8, 1), (6, 8), (12, 8), (127, 1), (16, 8)])
+def test_single_tokens_leave_no_quarter_of_the_chip_idle(B, Hkv, rows):
+    """Few heads with long keys: their shares make blocks for at least 192 of 256 CUs."""
+    for dtype, D in ((1, 128), (0, 64)):
+        n = shares(B, Hkv * rows, Hkv, 1, 1 << 17, D, dtype)
+        assert 192 <= n * B * Hkv <= 8 * 256
+
+
+def test_single_tokens_shares():
+    """One share where the heads fill the chip by themselves or the keys are few; as many as their rounds
+    pay for in between."""
+    assert [shares(b, 32, 8, 1, 8192, 128, 1) for b in (12, 16, 20, 24, 32)] == [3, 2, 3, 1, 1]
+    assert shares(16, 12, 12, 1, 562, 64, 0) == 1 and shares(40, 32, 8, 1, 8192, 128, 1) > 1
+
+
 def test_numbers_out_of_range():
     q, k = T(2, 3, 4, 64), T(2, 5, 2, 64)
     for scale in (1e39, -1e39, 2.0 ** 121):  # float32 of these, times log2(e), is not finite
