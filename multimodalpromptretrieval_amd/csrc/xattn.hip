@@ -259,6 +259,26 @@ __device__ __forceinline__ float halves(float x, F f) {
   return f(__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 
+template <int CTRL>
+__device__ __forceinline__ float permuted(float x) {
+  return __builtin_bit_cast(
+      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+// the sum over neighbouring groups of LPR lanes, in all of them (no LDS: lane permutations)
+template <int LPR>
+__device__ __forceinline__ float group_add(float x) {
+  x += permuted<0xB1>(x);   // lane ^ 1
+  x += permuted<0x4E>(x);   // lane ^ 2
+  x += permuted<0x141>(x);  // mirrored in 8: the other four
+  if constexpr (LPR >= 16) x += permuted<0x140>(x);  // mirrored in 16: the other eight
+  if constexpr (LPR == 32) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+  }
+  return x;
+}
+
 // ---- staging -------------------------------------------------------------------------------------
 // A tile of ROWS rows from memory straight to LDS (no registers in between): starts the reads; they
 // have landed after landed() and a barrier.  A wave's call writes 64 neighbouring pieces, so the
@@ -330,6 +350,15 @@ __device__ __forceinline__ void span_words(uint32_t* words, const uint8_t* keep,
       words[(i >> 5) + 1] = (uint32_t)(on >> 32);
     }
   }
+}
+// the keys that a span of n (words in LDS) has, the same in every lane
+__device__ __forceinline__ int span_keys(const uint32_t* words, int n, int lane) {
+  static_assert(SPAN / 32 == 128, "two words a lane");
+  const int all = (n + SPAN_UNIT - 1) / SPAN_UNIT * (SPAN_UNIT / 32);
+  const int own = (lane < all ? __popc(words[lane]) : 0) +
+                  (lane + 64 < all ? __popc(words[lane + 64]) : 0);
+  const float sum = halves(group_add<32>((float)own), [](float x, float y) { return x + y; });
+  return __builtin_amdgcn_readfirstlane((int)sum);
 }
 template <int KT>
 __device__ __forceinline__ int next_tile(const uint32_t* words, int at, int last) {
@@ -476,19 +505,22 @@ struct Shape {
 };
 
 // Runs over the live tiles of the block's keys [k_lo, k_hi): for each, compute(K, V, the tile's
-// words).  ZERO_K: masked keys' rows of K become zeros as V's do.
+// words).  ZERO_K: masked keys' rows of K become zeros as V's do.  ready: the words of the first span are
+// there already.
 template <class T, class M, int DP, int WR, bool ZERO_K, class KAt, class VAt, class F>
 __device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* words,
                                           const uint8_t* keep, int64_t k_lo, int64_t k_hi, int D,
-                                          KAt k_at, VAt v_at, int t, int wave, int lane,
+                                          KAt k_at, VAt v_at, int t, int wave, int lane, bool ready,
                                           F compute) {
   typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
   constexpr int KT = S::KT;
   for (int64_t base = k_lo; base < k_hi; base += SPAN) {
-    __syncthreads();
-    span_words(words, keep, base, k_hi, t, 64 * NW);
-    __syncthreads();
+    if (base > k_lo || !ready) {
+      __syncthreads();
+      span_words(words, keep, base, k_hi, t, 64 * NW);
+      __syncthreads();
+    }
     const int last = (int)min((int64_t)SPAN, k_hi - base);
     const auto load = [&](char* lds, int at) {
       E* k = reinterpret_cast<E*>(lds);
@@ -544,7 +576,11 @@ __device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* word
 // ---- forward -------------------------------------------------------------------------------------
 // The running maximum follows the scores only when they pass it by more than 8 (in base 2): until
 // then exponentials up to 2^8 share the old base, and the sums need no rescaling.
-// FINE: P to 16 bits as an operand (bf16).
+// FINE: P to 16 bits as an operand (bf16).  Where one key carries a row, P's rounding reaches the output
+// and the backward's row sum at full size, where many do it averages out: at 2 keys, gradients 1.7
+// times as far off as their own rounding takes them, 1.45 times with P to 16 bits.  So few keys are
+// multiplied FINE (2048 rows x 256 keys, 96 heads of 64: 42 us against 36), and what counts are those
+// that the mask keeps, however far a batch is padded.
 //
 // What bounds it are the matrix cores and the vector work of the exponentials (16 a lane for each 32 x 32
 // scores), which overlap little: at D = 128 the matrix pipes are busy 40 % of the cycles and the
@@ -554,22 +590,18 @@ __device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* word
 // (700); in fp32, whose products take 16 times as long and hide the rest, 1022 us and 552 us (135 and
 // 125 of 154 TFLOP/s).
 template <class T, class M, int DP, int WR, bool FINE>
-__global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fwd_kernel(XArgs a) {
+__device__ __forceinline__ void xattn_fwd_block(const XArgs& a, const Job& j, const uint8_t* keep,
+                                                char* lds, char* lds1, uint32_t* words, int t,
+                                                int lane, int wave, bool ready) {
   typedef Shape<M, DP, WR> S;
   typedef typename M::elem E;
   constexpr int WK = S::WK, NU = S::NU, NC = DP / M::CHUNK;
-  __shared__ __align__(16) char lds[S::BYTES];
-  __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
-  __shared__ uint32_t words[SPAN / 32];
-  const int t = threadIdx.x, lane = t & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), wr = wave % WR, wk = wave / WR;
-  const Job j = job_longest_first(a, t);
+  const int wr = wave % WR, wk = wave / WR;
   const int row = (j.tile * WR + wr) * 32 + (lane & 31);
   const bool in = row < a.R;
   const RowAt ra = row_at(a, j.hk, in ? row : 0);
   const T* k = static_cast<const T*>(a.k) + j.b * a.k_bs + j.hk * a.k_hs;
   const T* v = static_cast<const T*>(a.v) + j.b * a.v_bs + j.hk * a.v_hs;
-  const uint8_t* keep = a.keep ? a.keep + j.b * a.keep_bs : nullptr;
   const auto k_at = [&](int64_t r) { return k + r * a.k_ls; };
   const auto v_at = [&](int64_t r) { return v + r * a.v_ls; };
   typename M::frag q[NC];
@@ -580,7 +612,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
   bool some = false;             // the block's share has a key
   const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
   for_tiles<T, M, DP, WR, false>(lds, lds1, words, keep, k_lo, k_hi, a.D, k_at, v_at, t, wave, lane,
-                                 [&](const E* ks, const E* vs, const uint32_t* on) {
+                                 ready, [&](const E* ks, const E* vs, const uint32_t* on) {
       some = true;
       const int u0 = wk * NU;
       uint32_t bits[NU], any = 0, all = ~0u;
@@ -671,6 +703,42 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fw
     a.lse[((int64_t)j.b * a.H + ra.h) * a.Lq + ra.i] = lse_of(m * a.c, l, some);
 }
 
+constexpr int FINE_KEYS = 256;
+template <class T, class M, int DP, int WR>
+__global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::FWD_OCC)) void xattn_fwd_kernel(XArgs a) {
+  typedef Shape<M, DP, WR> S;
+  __shared__ __align__(16) char lds[S::BYTES];
+  __shared__ __align__(16) char lds1[S::BUFS == 2 ? S::BYTES : 16];
+  __shared__ uint32_t words[SPAN / 32];
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const Job j = job_longest_first(a, t);
+  const uint8_t* keep = a.keep ? a.keep + j.b * a.keep_bs : nullptr;
+  bool fine = a.Lk <= FINE_KEYS, ready = false;
+  if constexpr (std::is_same_v<T, bf16>) {
+    if (keep && !fine) {
+      // a share of a long row may hold half of FINE_KEYS by itself: it is split at 256 keys at least
+      const int most = a.splits > 1 ? FINE_KEYS / 2 : FINE_KEYS;
+      const int64_t k_lo = (int64_t)j.split * a.per_split;
+      const int64_t k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
+      int kept = 0;
+      for (int64_t base = k_lo; base < k_hi && kept <= most; base += SPAN) {
+        __syncthreads();
+        span_words(words, keep, base, k_hi, t, 64 * NW);
+        __syncthreads();
+        kept += span_keys(words, (int)min((int64_t)SPAN, k_hi - base), lane);
+        ready = base == k_lo;
+      }
+      fine = kept <= most;
+    }
+    if (fine) {
+      xattn_fwd_block<T, M, DP, WR, true>(a, j, keep, lds, lds1, words, t, lane, wave, ready);
+      return;
+    }
+  }
+  xattn_fwd_block<T, M, DP, WR, false>(a, j, keep, lds, lds1, words, t, lane, wave, ready);
+}
+
 // The splits of a row: rescaled to their common maximum and summed in order.  A wave per row, whose
 // lanes read the splits' statistics side by side and then AHEAD of their rows at a time: the time is
 // the latency of these reads (1024 rows of 4 splits 4.8 us; one split after the other 8.7).
@@ -742,25 +810,6 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // before the mask is known made masked batches slower, 66 us against 60.)
 constexpr int FEW_WAVES = 8, FEW_AHEAD = 4;
 
-template <int CTRL>
-__device__ __forceinline__ float permuted(float x) {
-  return __builtin_bit_cast(
-      float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
-// the sum over neighbouring groups of LPR lanes, in all of them (no LDS: lane permutations)
-template <int LPR>
-__device__ __forceinline__ float group_add(float x) {
-  x += permuted<0xB1>(x);   // lane ^ 1
-  x += permuted<0x4E>(x);   // lane ^ 2
-  x += permuted<0x141>(x);  // mirrored in 8: the other four
-  if constexpr (LPR >= 16) x += permuted<0x140>(x);  // mirrored in 16: the other eight
-  if constexpr (LPR == 32) {
-    const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    x = __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
-  }
-  return x;
-}
 // f over the lanes that hold the same column of neighbouring groups of LPR, in all of them
 template <int LPR, class F>
 __device__ __forceinline__ float across(float x, F f) {
@@ -1100,7 +1149,7 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq
   f32x16 acc[DP / 32] = {};
   const int64_t k_lo = (int64_t)j.split * a.per_split, k_hi = min((int64_t)a.Lk, k_lo + a.per_split);
   for_tiles<T, M, DP, WR, true>(lds, lds1, words, keep, k_lo, k_hi, a.D, k_at, v_at, t, wave, lane,
-                                [&](const E* ks, const E* vs, const uint32_t* on) {
+                                false, [&](const E* ks, const E* vs, const uint32_t* on) {
 #pragma unroll
       for (int u = wk * NU; u < (wk + 1) * NU; ++u) {
         const uint32_t bits = __builtin_amdgcn_readfirstlane(on[u]);
@@ -1354,7 +1403,6 @@ __global__ __launch_bounds__(256) void xattn_sum_kernel(XArgs a, int kind) {
 }
 
 // ---- host ----------------------------------------------------------------------------------------
-constexpr int FINE_KEYS = 256;
 constexpr int FEW_ROWS = 8;  // rows of a key head that the single-token kernel takes
 
 // Blocks along one axis and shares of the other: where the tiles alone leave the chip idle, the
@@ -1563,14 +1611,7 @@ int xattn_forward(XArgs a, const XPlan& p, hipStream_t s) {
     typedef typename MmaOf<T>::type M;
     MPR_TRY(by_tile(a.D, p.fwd.nw, [&](auto dp, auto nw) -> int {
       constexpr int DP = dp, WR = nw;
-      // Where one key carries a row, P's rounding reaches the output and the backward's row sum at
-      // full size, where many do it averages out: at 2 keys, gradients 1.7 times as far off as their
-      // own rounding takes them, 1.45 times with P to 16 bits.  So few keys are multiplied FINE
-      // (2048 rows x 256 keys, 96 heads of 64: 42 us against 36).
-      if (std::is_same_v<T, bf16> && a.Lk <= FINE_KEYS)
-        xattn_fwd_kernel<T, M, DP, WR, std::is_same_v<T, bf16>><<<blocks, 64 * NW, 0, s>>>(a);
-      else
-        xattn_fwd_kernel<T, M, DP, WR, false><<<blocks, 64 * NW, 0, s>>>(a);
+      xattn_fwd_kernel<T, M, DP, WR><<<blocks, 64 * NW, 0, s>>>(a);
       MPR_LAUNCHED();
       return MPR_OK;
     }));

@@ -301,6 +301,22 @@ def test_cross_attention_ragged_batch(device, dtype):
             assert torch.equal(x, y[order])
 
 
+@pytest.mark.parametrize("B,H,Lq,D", [(4, 2, 300, 64), (4, 8, 700, 64), (4, 2, 300, 128),
+                                      (4, 4, 20, 72)])
+@pytest.mark.parametrize("Lk", [100, 600, 5000])
+def test_cross_attention_few_kept_keys_in_a_padded_batch(device, B, H, Lq, D, Lk):
+    """bf16 entries of few keys take their probabilities to 16 bits (2^-16 twice over: what the second
+    term's rounding and the sum's leave) however far the batch is padded and its keys are shared."""
+    g = gen(17)
+    q, k, v, dout = xattn_inputs(g, B, H, H, Lq, Lk, D, BF16)
+    keep = torch.zeros(B, Lk, dtype=torch.bool, device="cuda")
+    keep[0, Lk - 1] = keep[1, :2] = keep[2, ::(Lk + 2) // 3] = keep[3, 5:100] = True
+    out, _ = xattn_check(q, k, v, keep, 0.2, dout)
+    ref, bound = R.attention(q.float(), k.float(), v.float(), keep, 0.2)["out"]
+    size = R.attention(q.float(), k.float(), v.float().abs(), keep, 0.2)["out"][0]
+    R.check(out, ref, bound + R.SLACK * 2 * 2.0 ** -16 * size + R.rounded(ref, BF16), "out")
+
+
 @pytest.mark.parametrize("Lq", [1, 12])
 def test_cross_attention_odd_strides_of_single_dims(device, Lq):
     """A dimension of size 1 has whatever stride it came with; an odd one is nobody's address."""
