@@ -417,7 +417,7 @@ int mpr_gather_rows(const float* table, const int32_t* ids, int64_t n, int32_t d
 int mpr_embed_bwd(const float* dY, int32_t d, const int32_t* uniq, const int32_t* offs,
                   const int32_t* pos, int32_t n_uniq, float* dW, void* stream);
 
-/* ---- tensor operators for tuning and serving the reader (multimodalpromptretrieval_amd/ops.py;
+/* ---- tensor operators for readers of T5's kind (multimodalpromptretrieval_amd/ops.py;
  * no reference counterpart: the reference trains with torch's own) ------------------------------
  * dtype codes: 0 float32, 1 bfloat16, 2 float16; sums and statistics are 32 bits or wider.  All
  * workspaces are the caller's, sized by the *_workspace calls, and hold nothing between calls, so

@@ -142,7 +142,7 @@ __global__ __launch_bounds__(1024) void clip_finish_kernel(const double* partial
 }
 
 // The chunks from the last to the first: the norm's pass left the last ones in the caches.  222 M
-// gradients (two thirds fp32, the others bf16) into an fp32 buffer: three launches of 114 us, 4.9 TB/s
+// gradients (two thirds fp32, the others bf16) into an fp32 buffer: three launches of 114 us, 4.75 TB/s
 // read and written together, after 58 us each for the norm, 4.2 TB/s.
 __global__ __launch_bounds__(CLIP_THREADS) void clip_scale_kernel(ClipTable tab,
                                                                   const ClipState* st) {

@@ -584,11 +584,12 @@ __device__ __forceinline__ void for_tiles(char* lds0, char* lds1, uint32_t* word
 //
 // What bounds it are the matrix cores and the vector work of the exponentials (16 a lane for each 32 x 32
 // scores), which overlap little: at D = 128 the matrix pipes are busy 40 % of the cycles and the
-// vector pipes 43 %.  32 rows a wave hold Q, the scores and the sums in registers with two waves a
-// SIMD (three at D = 64); four waves along the rows read a staged tile of 64 keys four times.  4 x 16
-// heads over 4, 1024 x 4096 keys, D = 128 in bf16 156 to 175 us (790 to 880 TFLOP/s), D = 64 99 us
-// (700); in fp32, whose products take 16 times as long and hide the rest, 1022 us and 552 us (135 and
-// 125 of 154 TFLOP/s).
+// vector pipes 45 %, at D = 64 30 and 60 %.  32 rows a wave hold Q, the scores and the sums in registers
+// with two waves a SIMD (three at D = 64); four waves along the rows read a staged tile of 64 keys four
+// times.  4 x 16 heads over 4, 1024 x 4096 keys, D = 128 in bf16, in a graph, 154 to 174 us (790 to 890
+// TFLOP/s; profiled, where passes stand apart, 186 on average and 173 at least), D = 64 103 us
+// (670); in fp32, whose products take 16 times as long and hide the rest, 1030 us and 562 us (133 and
+// 122 of 154 TFLOP/s).
 template <class T, class M, int DP, int WR, bool FINE>
 __device__ __forceinline__ void xattn_fwd_block(const XArgs& a, const Job& j, const uint8_t* keep,
                                                 char* lds, char* lds1, uint32_t* words, int t,
@@ -1099,8 +1100,8 @@ __global__ __launch_bounds__(256) void xattn_delta_kernel(XArgs a) {
 // dQ: WR of the block's waves along the rows (32 each), the others along the staged keys.  Scores and
 // dP come from one pass over K and V by rows, dS goes on to the third product in registers, and delta
 // is formed from O and dO while the first tile is on its way.  Three products for two of the forward's,
-// bound as it is: 4 x 16 heads over 4, 1024 x 4096, D = 128 in bf16 209 to 224 us (920 to 990 TFLOP/s
-// of its 6 B H Lq Lk D, where a large product reaches 1072).
+// bound as it is: 4 x 16 heads over 4, 1024 x 4096, D = 128 in bf16 207 us in a graph, 234 profiled
+// (1000, 880 TFLOP/s of its 6 B H Lq Lk D, where a large product reaches 1072).
 template <class T, class M, int DP, int WR>
 __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq_kernel(XArgs a) {
   typedef Shape<M, DP, WR> S;
@@ -1193,8 +1194,8 @@ __global__ __launch_bounds__(64 * NW, (Shape<M, DP, WR>::BWD_OCC)) void xattn_dq
 // dK, dV: WC of the block's waves along the keys (32 each), the others along the staged rows, RT at a
 // time, over the rows of every head that shares the keys.  K and V are operands of every product and
 // dK and dV sums of all: at D = 128 V waits in LDS (V_LDS), the rest leaves two waves a SIMD in bf16
-// and one in fp32.  Four products: 4 x 16 heads over 4, 1024 x 4096, D = 128 in bf16 291 to 306 us (900 to
-// 940 TFLOP/s of its 8 B H Lq Lk D); with dQ in fp32 3683 us, 131 of 154 TFLOP/s.
+// and one in fp32.  Four products: 4 x 16 heads over 4, 1024 x 4096, D = 128 in bf16 276 us in a graph,
+// 319 profiled (1000, 860 TFLOP/s of its 8 B H Lq Lk D); with dQ in fp32 3750 us, 128 of 154 TFLOP/s.
 template <class M, int DP, int WC>
 struct DkvShape {
   typedef typename M::elem E;

@@ -1,9 +1,10 @@
-"""Tensor operators for tuning and serving the T5 reader on the device.
+"""Tensor operators for tuning and serving readers of T5's kind on the device.
 
 The framework's trainer (``train.py``) runs the reference's own step: fp32, teacher forcing, cross
-entropy.  These operators are for what a user builds next to it — tuning the reader on chosen and
-rejected answers, in bf16, on longer prompts — each a differentiable torch function over
-hand-written kernels of libmpr.so:
+entropy.  ``T5VisionModel`` trains by that loss alone: its logits carry no gradient (``sequence_logps``
+scores answers with them, as a reference model).  These operators are for a reader that a user
+writes in torch next to it, to tune it on chosen and rejected answers, in bf16, on longer
+prompts; each is a differentiable torch function over hand-written kernels of libmpr.so:
 
 * ``embed`` — scaled embedding lookup; its gradient sums the positions of each token, sorted on the
   device (``train.EmbedFn`` groups them on the host);
