@@ -9,10 +9,10 @@
 // once for the group and dK, dV sum the heads in registers: no atomics, the same bits every run.
 //
 // Matrix products: bf16 inputs on v_mfma_f32_32x32x16_bf16, float inputs on v_mfma_f32_32x32x2_f32
-// (exact fp32 products).  Half is for single tokens only: as matrix operands, half gradients would
-// leave half's range, so the caller computes them in float.  The products are arranged so that a tile's scores come out of the matrix core in the
-// lane order in which the next product takes them (scores transposed: lane = row, registers =
-// keys): probabilities go from one product to the next in registers, never through LDS.  P and dS
+// (exact fp32 products).  Half is for single tokens only: it has no matrix-core variant here, and the
+// caller computes it in float.  The products are arranged so that a tile's scores come out of the matrix
+// core in the lane order in which the next product takes them (scores transposed: lane = row, registers
+// = keys): probabilities go from one product to the next in registers, never through LDS.  P and dS
 // are rounded to bf16 as operands of the second products, as the inputs are; sums stay fp32.  Two
 // things keep the backward's differences dP - rowsum(dO O) exact where a row has few keys and they
 // cancel: the forward divides by the sum of the rounded P (its weights then add up to 1), and it
@@ -803,8 +803,8 @@ __global__ __launch_bounds__(256) void xattn_join_kernel(XArgs a) {
 // The keys and values are read once and that is all the time there is: no matrix core, and LDS only
 // for the mask's bits and the end.  LPR lanes read a key's row, 16 bytes each, so a wave reads 64 /
 // LPR keys at a time; each such group of lanes keeps its own running maximum, sum and output share
-// of every row (the maximum moves as the tiled kernel's does), and they are joined when the keys are done.  The wave's next FEW_AHEAD reads are on
-// their way while the present ones are computed.  32 x 8 key heads of 4 rows, 8192 keys, D = 128 in
+// of every row (the maximum moves as the tiled kernel's does), and they are joined when the keys are
+// done.  The wave's next FEW_AHEAD reads are on their way while the present ones are computed.  32 x 8 key heads of 4 rows, 8192 keys, D = 128 in
 // bf16: 190 us, 5.7 TB/s (with every lane taking every row's exponential 199, and 184 against 163 for
 // ragged lengths, where the longest head's blocks are bound by their vector work); 16 x 12 heads, 562
 // keys, D = 64 in fp32 9.6 us, half of it until the first keys are there.  (Reading the first keys
